@@ -26,6 +26,7 @@ extern "C" {
 #define LING_B200_MAX_TREE_ROWS 32   /* rows of one sequence's tree (kernels.cuh:107 kMaxStreamRows = 32)    */
 #define LING_B200_MAX_TREE_VARIANTS 32 /* kernels.cuh:118 kMaxTreeVariants                                   */
 #define LING_B200_MAX_ROWS 2048      /* packed rows of one step (all sequences)                              */
+#define LING_B200_KV4_MAX_SEQS 1024   /* sequences of one call on an NVFP4 KV cache                               */
 
 /* ------------------------------------------------------------------------------------------------ status */
 enum {
@@ -679,6 +680,78 @@ int ling_b200_draft_head_mask_mark(ling_b200_draft_head* h, int session, const i
  * selected [cap] (both may be NULL): the rows that were scored. */
 int ling_b200_draft_head_run_sparse(ling_b200_draft_head* h, int session, const float* x, int E, int anchor, int* cand, float* unary,
                                     float* scores, int* n_selected, int* selected);
+
+/* ------------------------------------------------------------------------------------------------ a decode layer in 4 bits
+ * No counterpart in the reference, whose decode path reads FP8 weights and a BF16 cache.  NVFP4 operands (E2M1 values two a byte,
+ * the first in the low nibble; one E4M3 scale per 16 values) for one token to a prompt's rows: a product with a few rows, a
+ * paged KV cache, attention over it.  Unlike the _host entry points these take DEVICE pointers and only enqueue on `stream` (a
+ * cudaStream_t; NULL = the default stream): they allocate nothing, wait for nothing and may be captured into a graph.  All
+ * pointers and the stream belong to `device`, which need not be the calling thread's current one.  A call that is refused
+ * launches nothing.  `err`, where there is one, is a device word or NULL: the first error that the kernels find (a page id out of
+ * range, a batch outside its bounds) is recorded there (it is never cleared by the library), the positions concerned are skipped. */
+enum { LING_B200_F32 = 0, LING_B200_BF16 = 1, LING_B200_F16 = 2 }; /* element types */
+
+/* y[m][n] = alpha * sum_k x[m][k] * w[n][k] (or += with accumulate) for M rows, 1 <= M <= 32; w as ling_b200_quantize_nvfp4_host leaves it
+ * (values [N][K/2], scales [N][K/16], K % 16 == 0; alpha carries the tensor scale).  x [M][ldx], y [M][ldy] of any two of the
+ * types above, ldx >= K, ldy >= N in elements; y must not overlap x.  x stays in its type (fp32 included: no activation
+ * quantizer, unlike ling_b200_prefill_gemm_nvfp4_host), sums are fp32, each y is rounded once.  The result of a row does not
+ * depend on the other rows. */
+int ling_b200_nvfp4_matvec(int device, const void* x, int x_type, long long ldx, int M, const uint8_t* values, const uint8_t* scales,
+                           float alpha, int N, int K, void* y, int y_type, long long ldy, int accumulate, void* stream);
+
+/* One layer's NVFP4 cache: K and V of a position and kv head are head_dim / 2 bytes of values and head_dim / 16 scale bytes.
+ * Page 0 is reserved (an unmapped table entry), ids 1..pages are usable, as in the FP8 pool.  The represented value is
+ * value * scale * k_scale (v_scale); both tensor scales are powers of two in [2^-30, 2^30], so a value is exact in BF16. */
+typedef struct ling_b200_kv4 {
+  uint8_t *k, *v;             /* [pages + 1][kv_heads][page_tokens][head_dim / 2], 16-byte aligned */
+  uint8_t *k_scales, *v_scales; /* [pages + 1][kv_heads][page_tokens][head_dim / 16] E4M3, 16-byte aligned */
+  const int* tables;          /* [slots][max_pages] page ids */
+  int kv_heads, head_dim;     /* head_dim 64, 128 or 256 */
+  int page_tokens;            /* 16, 32, 64 or 128 */
+  int pages, slots, max_pages;
+  float k_scale, v_scale;
+} ling_b200_kv4;
+/* The packed rows of a call: rows row0[s] .. row0[s+1] are sequence s, its row i stands at position pos[s] + i of the slot's table
+ * (ragged, a sequence may have none; rows from row0[seqs] on are padding and are left as they were).  Device arrays; the bounds
+ * are the host's: a sequence outside them is skipped and recorded in err. */
+typedef struct ling_b200_kv4_batch {
+  const int *row0, *slot, *pos; /* [seqs + 1], [seqs], [seqs] */
+  const int* rope_pos;          /* [rows] the rotary position of a row, or NULL: its position (a tree's rows: pos + depth) */
+  const uint32_t* anc;          /* [rows] or NULL: row i sees row j of its sequence when bit j is set (max_rows <= 32; the ancestor
+                                   masks of a step's packing); NULL: the rows up to itself */
+  int seqs, rows;               /* sequences; rows the arrays have room for */
+  int max_rows, max_context;    /* no sequence has more rows; pos + rows of no sequence is larger */
+} ling_b200_kv4_batch;
+/* [rows][heads][head_dim] with strides in elements, head_dim contiguous: a tensor of its own or a slice of a projection's rows. */
+typedef struct ling_b200_rows {
+  void* p;
+  long long row, head;
+} ling_b200_rows;
+
+/* Writes the rows' K, rotated, and V, as they are, into the cache, and rotates the rows' queries beside them (q and q_out with q_heads
+ * heads, or both NULL; q_out may be q).  The rotation is attn_prepare's: dims d and d + rotary_dim / 2 of the first rotary_dim
+ * dims (even, 0 = none) turn by rope_pos * theta^(-2 d / rotary_dim).  Per 16 dims the scale is E4M3(clamp(amax / 6, 2^-9, 448)) and
+ * a code the nearest, a value halfway between two the smaller magnitude (ling_b200_quantize_nvfp4_host's rule); the rotation
+ * of keys and every comparison are carried beyond fp32, so codes are those of the exact values.  A K or V vector with a value that is not
+ * finite (over its tensor scale, in fp32) is stored as NaN whole.  Two rows of one call must not share a position of the cache. */
+int ling_b200_kv4_append(int device, const ling_b200_kv4* cache, const ling_b200_kv4_batch* batch, int type, const ling_b200_rows* k,
+                         const ling_b200_rows* v, const ling_b200_rows* q, int q_heads, const ling_b200_rows* q_out, int rotary_dim,
+                         double theta, int* err, void* stream);
+/* The values that the cache holds at the rows' positions, [rows][kv_heads][head_dim] in `type` (exact in BF16 and fp32); k or v may be
+ * NULL. */
+int ling_b200_kv4_read(int device, const ling_b200_kv4* cache, const ling_b200_kv4_batch* batch, int type, const ling_b200_rows* k,
+                       const ling_b200_rows* v, int* err, void* stream);
+/* out[r][h] = softmax(scale * q[r][h] . K) V over the positions row r sees: [0, pos) of its sequence and its in-flight rows (anc, or
+ * those up to itself; a call must have appended them).  q head h reads kv head h / (q_heads / kv_heads).  q (BF16 or FP16) is
+ * already rotated; out has its type.  lse [rows][q_heads], or NULL: log of the sum of exp(scale * q . k).  A row that sees nothing
+ * has out 0 and lse -inf; NaN or infinities at positions a row does not see do not reach it.  `workspace` holds the partial
+ * results of contexts that are split over SMs: as many bytes as ling_b200_kv4_attention_workspace says for the same cache
+ * dims, batch bounds and q_heads, 16-byte aligned, zeroed once before its first use and then left alone; calls that may overlap
+ * on the GPU (other streams, graphs launched together) need one each. */
+size_t ling_b200_kv4_attention_workspace(const ling_b200_kv4* cache, const ling_b200_kv4_batch* batch, int q_heads);
+int ling_b200_kv4_attention(int device, const ling_b200_kv4* cache, const ling_b200_kv4_batch* batch, int type, const ling_b200_rows* q,
+                            int q_heads, float scale, const ling_b200_rows* out, float* lse, void* workspace, size_t workspace_bytes,
+                            int* err, void* stream);
 
 /* Device memory helpers for callers without a CUDA binding (tests): device count, and name of device 0. */
 int ling_b200_device_count(void);

@@ -760,3 +760,177 @@ def describe_tree(parent, chain):
     t = TreeDesc()
     rc = lib().ling_b200_describe_tree(_ip(par), len(par), chain, C.byref(t))
     return rc, t
+
+
+# ---- a decode layer in 4 bits: operators on DEVICE arrays (anything with data_ptr, shape, stride, dtype and device, as a torch
+# tensor has).  They enqueue on `stream` (a cudaStream_t as an integer; 0 = the default stream) and return.
+F32, BF16, F16 = range(3)
+_ELEMENT = {"torch.float32": F32, "torch.bfloat16": BF16, "torch.float16": F16}
+KV4_MAX_SEQS = 1024
+
+
+class _Kv4(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("k_scales", C.c_void_p), ("v_scales", C.c_void_p), ("tables", C.c_void_p),
+                ("kv_heads", C.c_int), ("head_dim", C.c_int), ("page_tokens", C.c_int), ("pages", C.c_int), ("slots", C.c_int),
+                ("max_pages", C.c_int), ("k_scale", C.c_float), ("v_scale", C.c_float)]
+
+
+class _Kv4Batch(C.Structure):
+    _fields_ = [("row0", C.c_void_p), ("slot", C.c_void_p), ("pos", C.c_void_p), ("rope_pos", C.c_void_p), ("anc", C.c_void_p),
+                ("seqs", C.c_int), ("rows", C.c_int), ("max_rows", C.c_int), ("max_context", C.c_int)]
+
+
+class _Rows(C.Structure):
+    _fields_ = [("p", C.c_void_p), ("row", C.c_longlong), ("head", C.c_longlong)]
+
+
+def _refuse(what):
+    raise LingError("%s failed (status %d)" % (what, ERR_ARG))
+
+
+def _device_of(a, what):
+    if not hasattr(a, "data_ptr") or a.device.type != "cuda":
+        _refuse(what + ": a device array expected")
+    return a.device.index or 0
+
+
+def _words(a, n, what, device, optional=False):
+    """The address of a contiguous device array of at least n 32-bit integers."""
+    if a is None and optional:
+        return None
+    if _device_of(a, what) != device or a.element_size() != 4 or a.is_floating_point() or not a.is_contiguous() or a.numel() < n:
+        _refuse("%s: a contiguous array of at least %d 32-bit integers on device %d expected" % (what, n, device))
+    return a.data_ptr()
+
+
+def _bytes(a, shape, what, device):
+    if _device_of(a, what) != device or a.element_size() != 1 or not a.is_contiguous() or tuple(a.shape) != tuple(shape):
+        _refuse("%s: a contiguous byte array %s on device %d expected" % (what, tuple(shape), device))
+    return a.data_ptr()
+
+
+def _matrix(a, what, device):
+    """(address, element type, row stride) of a device matrix with contiguous rows."""
+    t = _ELEMENT.get(str(a.dtype))
+    if t is None or _device_of(a, what) != device or a.dim() != 2 or (a.shape[1] > 1 and a.stride(1) != 1):
+        _refuse("%s: a matrix of float32, bfloat16 or float16 with contiguous rows on device %d expected" % (what, device))
+    return a.data_ptr(), t, a.stride(0) if a.shape[0] > 1 else max(a.shape[1], 1)
+
+
+def _rows_of(a, rows, heads, dim, dtype, what, device):
+    """[rows][heads][dim] with a contiguous last dimension as the C structure."""
+    shape, stride = a.shape, a.stride()
+    if _device_of(a, what) != device or a.dtype != dtype or len(shape) != 3 or shape[0] < rows or shape[1] != heads or shape[2] != dim or stride[2] != 1:
+        _refuse("%s: an array [%d][%d][%d] of %s with a contiguous last dimension on device %d expected" % (what, rows, heads, dim, dtype, device))
+    return C.byref(_Rows(a.data_ptr(), stride[0] if shape[0] > 1 else heads * max(stride[1], dim), stride[1] if heads > 1 else dim))
+
+
+_MATVEC_ARGS = [C.c_int, C.c_void_p, C.c_int, C.c_longlong, C.c_int, C.c_void_p, C.c_void_p, C.c_float, C.c_int, C.c_int, C.c_void_p, C.c_int,
+                C.c_longlong, C.c_int, C.c_void_p]
+
+
+def nvfp4_matvec(x, values, scales, alpha, y, accumulate=False, stream=0):
+    """y = alpha * x . w^T (or += with accumulate) for x [M][K], 1 <= M <= 32 rows of float32, bfloat16 or float16, and the NVFP4 weight
+    values [N][K/2], scales [N][K/16] (bytes, as quantize_nvfp4 gives them; alpha carries the tensor scale).  y [M][N] of any of
+    the three types.  ling_b200_nvfp4_matvec."""
+    device = _device_of(values, "nvfp4_matvec values")
+    xp, xt, ldx = _matrix(x, "nvfp4_matvec x", device)
+    yp, yt, ldy = _matrix(y, "nvfp4_matvec y", device)
+    M, K = x.shape
+    N = values.shape[0]
+    if y.shape[0] != M or y.shape[1] != N or K % 16:
+        _refuse("nvfp4_matvec: x [M][K], values [N][K/2], y [M][N] with K a multiple of 16 expected")
+    fn = lib().ling_b200_nvfp4_matvec
+    if fn.argtypes is None:
+        fn.argtypes = _MATVEC_ARGS
+    check(fn(device, xp, xt, ldx, M, _bytes(values, (N, K // 2), "nvfp4_matvec values", device), _bytes(scales, (N, K // 16), "nvfp4_matvec scales", device),
+             alpha, N, K, yp, yt, ldy, 1 if accumulate else 0, stream), "nvfp4_matvec")
+
+
+class Kv4Batch:
+    """The packed rows of a call on an NVFP4 cache (ling_b200_kv4_batch): device arrays row0 [seqs + 1], slot and pos [seqs]; rows the arrays
+    have room for, max_rows and max_context bounds on one sequence's rows and on pos + rows; anc [rows] ancestor masks, rope_pos
+    [rows] rotary positions.  Keeps the arrays alive; their contents may change between calls."""
+
+    def __init__(self, row0, slot, pos, rows, max_rows, max_context, anc=None, rope_pos=None):
+        self.device = _device_of(row0, "Kv4Batch row0")
+        self.arrays = (row0, slot, pos, rope_pos, anc)
+        seqs = slot.shape[0]
+        self.c = _Kv4Batch(_words(row0, seqs + 1, "Kv4Batch row0", self.device), _words(slot, seqs, "Kv4Batch slot", self.device),
+                           _words(pos, seqs, "Kv4Batch pos", self.device), _words(rope_pos, rows, "Kv4Batch rope_pos", self.device, True),
+                           _words(anc, rows, "Kv4Batch anc", self.device, True), seqs, rows, max_rows, max_context)
+        self.ref = C.byref(self.c)
+
+
+class Kv4Cache:
+    """One layer's paged NVFP4 cache (ling_b200_kv4) over device arrays the caller owns: k, v [pages + 1][kv_heads][page_tokens][head_dim / 2],
+    k_scales, v_scales [..][head_dim / 16] bytes, tables [slots][max_pages] page ids; k_scale, v_scale powers of two."""
+
+    def __init__(self, k, k_scales, v, v_scales, tables, k_scale=1.0, v_scale=1.0):
+        self.device = _device_of(k, "Kv4Cache k")
+        self.arrays = (k, k_scales, v, v_scales, tables)
+        if k.dim() != 4 or tables.dim() != 2:
+            _refuse("Kv4Cache: k [pages + 1][kv_heads][page_tokens][head_dim / 2] and tables [slots][max_pages] expected")
+        n, self.kv_heads, page_tokens, half = k.shape
+        self.head_dim = 2 * half
+        codes, scales = (n, self.kv_heads, page_tokens, half), (n, self.kv_heads, page_tokens, half // 8)
+        self.c = _Kv4(_bytes(k, codes, "Kv4Cache k", self.device), _bytes(v, codes, "Kv4Cache v", self.device),
+                      _bytes(k_scales, scales, "Kv4Cache k_scales", self.device), _bytes(v_scales, scales, "Kv4Cache v_scales", self.device),
+                      _words(tables, 1, "Kv4Cache tables", self.device), self.kv_heads, self.head_dim, page_tokens, n - 1, tables.shape[0], tables.shape[1],
+                      k_scale, v_scale)
+        self.ref = C.byref(self.c)
+        L = lib()
+        self._append, self._read, self._attention = L.ling_b200_kv4_append, L.ling_b200_kv4_read, L.ling_b200_kv4_attention
+        v_, i_ = C.c_void_p, C.c_int
+        self._append.argtypes = [i_, v_, v_, i_, v_, v_, v_, i_, v_, i_, C.c_double, v_, v_]
+        self._read.argtypes = [i_, v_, v_, i_, v_, v_, v_, v_]
+        self._attention.argtypes = [i_, v_, v_, i_, v_, i_, C.c_float, v_, v_, v_, C.c_size_t, v_, v_]
+        L.ling_b200_kv4_attention_workspace.restype = C.c_size_t
+        L.ling_b200_kv4_attention_workspace.argtypes = [v_, v_, i_]
+
+    def _rows(self, batch, a, heads, dtype, what):
+        if batch.device != self.device:
+            _refuse(what + ": the batch and the cache are on different devices")
+        return None if a is None else _rows_of(a, batch.c.rows, heads, self.head_dim, dtype, what, self.device)
+
+    def _type(self, a, what):
+        t = _ELEMENT.get(str(a.dtype))
+        if t is None:
+            _refuse(what + ": float32, bfloat16 or float16 expected")
+        return t
+
+    def append(self, batch, k, v, q=None, q_out=None, rotary_dim=0, theta=1e7, err=None, stream=0):
+        """Writes the rows' k, rotated, and v into the cache and rotates q into q_out ([rows][heads][head_dim] each; ling_b200_kv4_append)."""
+        heads = 0 if q is None else q.shape[1]
+        check(self._append(self.device, self.ref, batch.ref, self._type(k, "append k"), self._rows(batch, k, self.kv_heads, k.dtype, "append k"),
+                           self._rows(batch, v, self.kv_heads, k.dtype, "append v"), self._rows(batch, q, heads, k.dtype, "append q"), heads,
+                           self._rows(batch, q_out, heads, k.dtype, "append q_out"), rotary_dim, theta, _words(err, 1, "append err", self.device, True),
+                           stream), "kv4_append")
+
+    def read(self, batch, k=None, v=None, err=None, stream=0):
+        """The values held at the rows' positions into k and v [rows][kv_heads][head_dim] (either may be None; ling_b200_kv4_read)."""
+        any_ = k if k is not None else v
+        if any_ is None:
+            _refuse("read: k or v expected")
+        check(self._read(self.device, self.ref, batch.ref, self._type(any_, "read"), self._rows(batch, k, self.kv_heads, any_.dtype, "read k"),
+                         self._rows(batch, v, self.kv_heads, any_.dtype, "read v"), _words(err, 1, "read err", self.device, True), stream), "kv4_read")
+
+    def attention_workspace_bytes(self, batch, q_heads):
+        """Bytes of the workspace that attention() needs with this batch's bounds (zeroed once by the caller)."""
+        n = lib().ling_b200_kv4_attention_workspace(self.ref, batch.ref, q_heads)
+        if n == 0:
+            raise LingError("kv4_attention_workspace failed (status %d): %s" % (ERR_ARG, last_error()))
+        return n
+
+    def attention(self, batch, q, out, scale, workspace, lse=None, err=None, stream=0):
+        """Attention of the rows' rotated q [rows][q_heads][head_dim] over the cache into out (its type, bfloat16 or float16); lse
+        [rows][q_heads] float32 (ling_b200_kv4_attention)."""
+        heads = q.shape[1]
+        if _device_of(workspace, "attention workspace") != self.device or not workspace.is_contiguous():
+            _refuse("attention: a contiguous workspace on device %d expected" % self.device)
+        if lse is not None and (_device_of(lse, "attention lse") != self.device or str(lse.dtype) != "torch.float32" or not lse.is_contiguous() or
+                                lse.numel() < batch.c.rows * heads):
+            _refuse("attention: lse [rows][q_heads] of float32 expected")
+        check(self._attention(self.device, self.ref, batch.ref, self._type(q, "attention q"), self._rows(batch, q, heads, q.dtype, "attention q"), heads, scale,
+                              self._rows(batch, out, heads, q.dtype, "attention out"), None if lse is None else lse.data_ptr(), workspace.data_ptr(),
+                              workspace.numel() * workspace.element_size(), _words(err, 1, "attention err", self.device, True), stream), "kv4_attention")

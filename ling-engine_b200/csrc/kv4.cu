@@ -1,0 +1,309 @@
+// kv4.cu -- writing and reading a paged NVFP4 KV cache: ling_b200_kv4_append, ling_b200_kv4_read.
+//
+// append, of a vector x of head_dim values (a key after its rotation, a value as it is), per group g of 16 dims:
+//   s = E4M3(clamp(max |x| / 6, 2^-9, 448)),  code = the E2M1 value nearest x / s, halfway to the smaller magnitude.
+// x / s lies above a border b exactly when |x| > b * s, and b * s (3 + 4 significant bits) is exact in fp32, so the codes are
+// found by comparisons alone.  A key's rotation is carried in double and brought to fp32 by rounding to odd (the last bit set
+// when anything was cut off), which keeps every comparison with a value of fewer bits what it is for the exact number: codes
+// do not depend on how fp32 would have rounded the rotation.  Queries need no such care and turn in fp32.
+#include "decode4.cuh"
+
+namespace lb {
+namespace d4 {
+
+bool kv4_cache_ok(const ling_b200_kv4* c, const char* who) {
+  auto no = [&](const char* why) {
+    set_error(std::string(who) + ": " + why);
+    return false;
+  };
+  if (!c || !c->k || !c->v || !c->k_scales || !c->v_scales || !c->tables) return no("null cache pointer");
+  if (!aligned(c->k, 16) || !aligned(c->v, 16) || !aligned(c->k_scales, 16) || !aligned(c->v_scales, 16) || !aligned(c->tables, 4))
+    return no("the cache's arrays must start on 16-byte boundaries");
+  if (c->head_dim != 64 && c->head_dim != 128 && c->head_dim != 256) return no("head_dim must be 64, 128 or 256");
+  if (c->page_tokens != 16 && c->page_tokens != 32 && c->page_tokens != 64 && c->page_tokens != 128)
+    return no("page_tokens must be 16, 32, 64 or 128");
+  if (c->kv_heads < 1 || c->kv_heads > 1024 || c->pages < 1 || c->slots < 1 || c->max_pages < 1 ||
+      c->max_pages > (1 << 30) / c->page_tokens)
+    return no("a cache size out of range");
+  for (float s : {c->k_scale, c->v_scale}) {
+    int e = 0;
+    if (!(s >= 0x1p-30f && s <= 0x1p30f) || std::frexp(s, &e) != 0.5f) return no("k_scale and v_scale must be powers of two in [2^-30, 2^30]");
+  }
+  return true;
+}
+
+bool kv4_batch_ok(const ling_b200_kv4* c, const ling_b200_kv4_batch* b, const char* who) {
+  auto no = [&](const char* why) {
+    set_error(std::string(who) + ": " + why);
+    return false;
+  };
+  if (!b || !b->row0 || !b->slot || !b->pos) return no("null batch pointer");
+  if (!aligned(b->row0, 4) || !aligned(b->slot, 4) || !aligned(b->pos, 4) || !aligned(b->rope_pos, 4) || !aligned(b->anc, 4))
+    return no("a batch array is not aligned");
+  if (b->seqs < 1 || b->seqs > LING_B200_KV4_MAX_SEQS) return no("seqs out of range");
+  if (b->rows < 0 || b->rows > (1 << 24) || b->max_rows < 0 || b->max_rows > b->rows) return no("rows or max_rows out of range");
+  if (b->anc && b->max_rows > LING_B200_MAX_TREE_ROWS) return no("ancestor masks hold 32 rows of a sequence");
+  if (b->max_context < b->max_rows || (long long)b->max_context > (long long)c->max_pages * c->page_tokens)
+    return no("max_context is below max_rows or beyond the page tables");
+  return true;
+}
+
+bool kv4_rows_ok(const ling_b200_rows* r, int type, int heads, int dim, const char* who, const char* what) {
+  if (!r || !r->p || !aligned(r->p, type_size(type)) || r->head < dim || r->row < dim) {
+    set_error(std::string(who) + ": bad rows (" + what + "): a pointer aligned to its type and strides of at least head_dim expected");
+    return false;
+  }
+  return true;
+}
+
+bool kv4_out_ok(const ling_b200_rows* r, int type, int rows, int heads, int dim, const char* who, const char* what) {
+  if (!kv4_rows_ok(r, type, heads, dim, who, what)) return false;
+  const bool apart = r->head <= r->row ? r->row >= (heads - 1) * r->head + dim : r->head >= (rows - 1) * r->row + dim;
+  if (!apart) set_error(std::string(who) + ": the rows of " + what + " overlap");
+  return apart;
+}
+
+}  // namespace d4
+namespace {
+using namespace d4;
+
+constexpr int kThreads = 256;
+
+// fp32 with the last bit set when d is not an fp32 value (rounding to odd).
+__device__ __forceinline__ float round_to_odd(double d) {
+  const float f = __double2float_rz(d);
+  return double(f) == d ? f : __uint_as_float(__float_as_uint(f) | 1u);
+}
+
+// Eight codes of x[0..8) under the scale s, the first in the low nibble.
+__device__ __forceinline__ uint32_t e2m1_codes(const float* x, float s) {
+  const float b0 = 0.25f * s, b1 = 0.75f * s, b2 = 1.25f * s, b3 = 1.75f * s, b4 = 2.5f * s, b5 = 3.5f * s, b6 = 5.f * s;
+  uint32_t w = 0;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const float a = fabsf(x[j]);
+    const bool hi = a > b3;                         // codes 4..7 or 0..3
+    const bool mid = a > (hi ? b5 : b1);
+    const bool lo = a > (hi ? (mid ? b6 : b4) : (mid ? b2 : b0));
+    w |= ((hi ? 4u : 0u) | (mid ? 2u : 0u) | (lo ? 1u : 0u) | (__float_as_uint(x[j]) >> 31 << 3)) << (4 * j);
+  }
+  return w;
+}
+
+struct AppendArgs {
+  ling_b200_kv4 c;
+  ling_b200_kv4_batch b;
+  ling_b200_rows k, v, q, q_out;
+  int q_heads, rot;
+  double theta;
+  int* err;
+};
+
+// A block per packed row; a thread per group of 16 dims of one head's K, V or query vector (the groups of a vector are
+// neighbouring lanes of one warp).  Floor: the rows read and 9 / 16 byte a value written.
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(kThreads) kv4_append_kernel(AppendArgs a) {
+  pdl_sync();  // first statement: see common.cuh
+  __shared__ double2 turn[128];  // cos, sin of the row's angles
+  __shared__ float2 turn32[128];
+  const int r = blockIdx.x, tid = threadIdx.x, lane = tid & 31;
+  const int s = kv4_find_seq(a.b.row0, a.b.seqs, r);
+  if (s < 0) return;  // padding behind the last sequence
+  const Kv4Seq q = kv4_seq(a.c, a.b, s);
+  const int pos = q.pos + r - q.row0, D = a.c.head_dim, groups = D / 16, T_page = a.c.page_tokens;
+  int page = 0;
+  if (q.ok) page = a.c.tables[size_t(q.slot) * a.c.max_pages + pos / T_page];
+  if (!q.ok || page < 1 || page > a.c.pages) {
+    if (tid == 0) dev_fail(a.err, q.ok ? int(kDevBadPage) : kDevBadBatch);
+    return;
+  }
+  const int half = a.rot / 2;
+  const int rp = a.b.rope_pos ? a.b.rope_pos[r] : pos;
+  for (int i = tid; i < half; i += kThreads) {
+    double sn, cs;
+    sincos(double(rp) * pow(a.theta, -2.0 * i / a.rot), &sn, &cs);
+    turn[i] = make_double2(cs, sn), turn32[i] = make_float2(float(cs), float(sn));
+  }
+  __syncthreads();
+  const int n_kv = a.c.kv_heads * groups, tasks = 2 * n_kv + a.q_heads * groups;
+  for (int t0 = 0; t0 < tasks; t0 += kThreads) {
+    const int t = t0 + tid;
+    if (t - lane >= tasks) break;  // whole warps: the lanes of a warp exchange below
+    const bool live = t < tasks, is_v = t >= n_kv && t < 2 * n_kv, is_q = t >= 2 * n_kv;
+    const int u = is_q ? t - 2 * n_kv : is_v ? t - n_kv : t, head = u / groups, g = u % groups;
+    const ling_b200_rows& src = is_q ? a.q : is_v ? a.v : a.k;
+    const T* vec = static_cast<const T*>(src.p) + r * src.row + head * src.head;
+    float x[16] = {};
+    bool bad = false;
+    float amax6 = 0.f;  // max |x| / 6
+    if (live) {
+      load16<T, VEC>(vec + g * 16, x);
+      if (!is_v && g * 16 < a.rot) {
+        float o[16];  // the dims these turn with
+        const bool whole = half % 16 == 0;
+        if (whole) {
+          load16<T, VEC>(vec + (g * 16 < half ? g * 16 + half : g * 16 - half), o);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            const int d = g * 16 + j;
+            o[j] = d < a.rot ? to_f32<T>(vec[d < half ? d + half : d - half]) : 0.f;
+          }
+        }
+        const double inv = 1.0 / double(a.c.k_scale);
+        double top = 0.0;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          const int d = g * 16 + j;
+          if (d >= a.rot) {
+            if (!is_q) x[j] *= float(inv), top = fmax(top, fabs(double(x[j]))), bad |= !isfinite(x[j]);
+            continue;
+          }
+          const int i = d < half ? d : d - half;
+          if (is_q) {
+            const float2 cs = turn32[i];
+            x[j] = d < half ? x[j] * cs.x - o[j] * cs.y : x[j] * cs.x + o[j] * cs.y;
+          } else {
+            const double2 cs = turn[i];
+            const double z = (d < half ? double(x[j]) * cs.x - double(o[j]) * cs.y : double(x[j]) * cs.x + double(o[j]) * cs.y) * inv;
+            bad |= !(fabs(z) <= 3.402823e38);
+            top = fmax(top, fabs(z));
+            x[j] = round_to_odd(z);
+          }
+        }
+        amax6 = float(top / 6.0);
+      } else if (!is_q) {
+        const float inv = 1.f / (is_v ? a.c.v_scale : a.c.k_scale);
+        float top = 0.f;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          x[j] *= inv;
+          bad |= !isfinite(x[j]);
+          top = fmaxf(top, fabsf(x[j]));
+        }
+        amax6 = __fdiv_rn(top, 6.f);
+      }
+    }
+    // a vector with a value that is not finite is NaN whole; the ballot also keeps a query's stores behind all loads of its vector
+    const unsigned any = __ballot_sync(0xffffffffu, bad) >> (lane / groups * groups) & ((1u << groups) - 1u);
+    if (!live) continue;
+    if (is_q) {
+      store16<T, VEC>(static_cast<T*>(a.q_out.p) + r * a.q_out.row + head * a.q_out.head + g * 16, x);
+      continue;
+    }
+    const size_t at = kv4_vector(a.c, page, head, pos % T_page);
+    uint8_t code = to_e4m3(fminf(fmaxf(amax6, 0x1p-9f), 448.f));
+    const float sc = from_e4m3(code);
+    uint2 w = make_uint2(e2m1_codes(x, sc), e2m1_codes(x + 8, sc));
+    if (any) w = make_uint2(0, 0), code = 0x7f;
+    reinterpret_cast<uint2*>((is_v ? a.c.v : a.c.k) + at * (D / 2))[g] = w;
+    (is_v ? a.c.v_scales : a.c.k_scales)[at * groups + g] = code;
+  }
+}
+
+struct ReadArgs {
+  ling_b200_kv4 c;
+  ling_b200_kv4_batch b;
+  ling_b200_rows k, v;
+  int* err;
+};
+
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(kThreads) kv4_read_kernel(ReadArgs a) {
+  pdl_sync();  // first statement: see common.cuh
+  const int r = blockIdx.x;
+  const int s = kv4_find_seq(a.b.row0, a.b.seqs, r);
+  if (s < 0) return;
+  const Kv4Seq q = kv4_seq(a.c, a.b, s);
+  const int pos = q.pos + r - q.row0, D = a.c.head_dim, groups = D / 16, T_page = a.c.page_tokens, n_kv = a.c.kv_heads * groups;
+  int page = 0;
+  if (q.ok) page = a.c.tables[size_t(q.slot) * a.c.max_pages + pos / T_page];
+  if (!q.ok || page < 1 || page > a.c.pages) {
+    if (threadIdx.x == 0) dev_fail(a.err, q.ok ? int(kDevBadPage) : kDevBadBatch);
+    return;
+  }
+  for (int t = threadIdx.x; t < 2 * n_kv; t += kThreads) {
+    const bool is_v = t >= n_kv;
+    const int u = is_v ? t - n_kv : t, head = u / groups, g = u % groups;
+    const ling_b200_rows& to = is_v ? a.v : a.k;
+    if (!to.p) continue;
+    const size_t at = kv4_vector(a.c, page, head, pos % T_page);
+    float x[16];
+    decode16(reinterpret_cast<const uint2*>((is_v ? a.c.v : a.c.k) + at * (D / 2))[g],
+             from_e4m3((is_v ? a.c.v_scales : a.c.k_scales)[at * groups + g]) * (is_v ? a.c.v_scale : a.c.k_scale), x);
+    store16<T, VEC>(static_cast<T*>(to.p) + r * to.row + head * to.head + g * 16, x);
+  }
+}
+
+DeviceInfo g_devices[kMaxDevices];
+std::mutex g_mutex;
+
+template <typename T>
+int append_launch(const AppendArgs& a, bool vec, cudaStream_t s) {
+  LB_CUDA(launch_kernel(vec ? kv4_append_kernel<T, true> : kv4_append_kernel<T, false>, dim3(a.b.rows), dim3(kThreads), size_t(0), s, a));
+  LB_LAUNCH("kv4_append_kernel");
+  return LING_B200_OK;
+}
+template <typename T>
+int read_launch(const ReadArgs& a, bool vec, cudaStream_t s) {
+  LB_CUDA(launch_kernel(vec ? kv4_read_kernel<T, true> : kv4_read_kernel<T, false>, dim3(a.b.rows), dim3(kThreads), size_t(0), s, a));
+  LB_LAUNCH("kv4_read_kernel");
+  return LING_B200_OK;
+}
+
+}  // namespace
+}  // namespace lb
+
+using namespace lb;
+using namespace lb::d4;
+
+extern "C" int ling_b200_kv4_append(int device, const ling_b200_kv4* cache, const ling_b200_kv4_batch* batch, int type,
+                                    const ling_b200_rows* k, const ling_b200_rows* v, const ling_b200_rows* q, int q_heads,
+                                    const ling_b200_rows* q_out, int rotary_dim, double theta, int* err, void* stream) {
+  const char* who = "kv4_append";
+  if (!kv4_cache_ok(cache, who) || !kv4_batch_ok(cache, batch, who)) return LING_B200_ERR_ARG;
+  if (!type_ok(type)) {
+    set_error("kv4_append: element types are LING_B200_F32, _BF16 and _F16");
+    return LING_B200_ERR_ARG;
+  }
+  const int D = cache->head_dim;
+  if (!kv4_rows_ok(k, type, cache->kv_heads, D, who, "k") || !kv4_rows_ok(v, type, cache->kv_heads, D, who, "v")) return LING_B200_ERR_ARG;
+  if (!q != !q_out || (q && (q_heads < 1 || q_heads > 1024 || !kv4_rows_ok(q, type, q_heads, D, who, "q") || !kv4_out_ok(q_out, type, batch->rows, q_heads, D, who, "q_out")))) {
+    if (!q != !q_out || q_heads < 1 || q_heads > 1024) set_error("kv4_append: q and q_out come together, with 1 to 1024 heads");
+    return LING_B200_ERR_ARG;
+  }
+  if (rotary_dim < 0 || rotary_dim > D || rotary_dim % 2 != 0 || !(theta > 0.0) || !std::isfinite(theta) || !aligned(err, 4)) {
+    set_error("kv4_append: rotary_dim must be even and at most head_dim, theta positive and finite");
+    return LING_B200_ERR_ARG;
+  }
+  if (batch->rows == 0) return LING_B200_OK;
+  DeviceGuard guard;
+  int sms = 0;
+  if (const int r = enter_device(guard, device, g_devices, g_mutex, [] { return LING_B200_OK; }, &sms)) return r;
+  AppendArgs a{*cache, *batch, *k, *v, {nullptr, 0, 0}, {nullptr, 0, 0}, 0, rotary_dim, theta, err};
+  bool vec = rows_vec(*k, type) && rows_vec(*v, type) && (rotary_dim / 2 % 16 != 0 || rotary_dim / 2 * type_size(type) % 16 == 0);
+  if (q) a.q = *q, a.q_out = *q_out, a.q_heads = q_heads, vec = vec && rows_vec(*q, type) && rows_vec(*q_out, type);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  return type == LING_B200_F32 ? append_launch<float>(a, vec, s) : type == LING_B200_BF16 ? append_launch<__nv_bfloat16>(a, vec, s) : append_launch<__half>(a, vec, s);
+}
+
+extern "C" int ling_b200_kv4_read(int device, const ling_b200_kv4* cache, const ling_b200_kv4_batch* batch, int type, const ling_b200_rows* k,
+                                  const ling_b200_rows* v, int* err, void* stream) {
+  const char* who = "kv4_read";
+  if (!kv4_cache_ok(cache, who) || !kv4_batch_ok(cache, batch, who)) return LING_B200_ERR_ARG;
+  if (!type_ok(type) || (!k && !v) || !aligned(err, 4)) {
+    set_error("kv4_read: a type and k or v expected");
+    return LING_B200_ERR_ARG;
+  }
+  if ((k && !kv4_out_ok(k, type, batch->rows, cache->kv_heads, cache->head_dim, who, "k")) ||
+      (v && !kv4_out_ok(v, type, batch->rows, cache->kv_heads, cache->head_dim, who, "v")))
+    return LING_B200_ERR_ARG;
+  if (batch->rows == 0) return LING_B200_OK;
+  DeviceGuard guard;
+  int sms = 0;
+  if (const int r = enter_device(guard, device, g_devices, g_mutex, [] { return LING_B200_OK; }, &sms)) return r;
+  const ReadArgs a{*cache, *batch, k ? *k : ling_b200_rows{nullptr, 0, 0}, v ? *v : ling_b200_rows{nullptr, 0, 0}, err};
+  const bool vec = (!k || rows_vec(*k, type)) && (!v || rows_vec(*v, type));
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  return type == LING_B200_F32 ? read_launch<float>(a, vec, s) : type == LING_B200_BF16 ? read_launch<__nv_bfloat16>(a, vec, s) : read_launch<__half>(a, vec, s);
+}
