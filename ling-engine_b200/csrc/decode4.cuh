@@ -83,6 +83,13 @@ __device__ __forceinline__ uint32_t e2m1x2_to_h2(uint32_t byte) {
   asm("{\n .reg .b8 b;\n mov.b16 {b, _}, %1;\n cvt.rn.f16x2.e2m1x2 %0, b;\n}" : "=r"(r) : "h"(uint16_t(byte)));
   return r;
 }
+// Eight codes of a word as four pairs of halves, exactly (half the rate of an fp32 operation on B200, a third of what shifts and masks cost).
+__device__ __forceinline__ void e2m1x8_to_h2(uint32_t w, uint32_t (&h)[4]) {
+  asm("{\n .reg .b8 a, b, c, d;\n mov.b32 {a, b, c, d}, %4;\n cvt.rn.f16x2.e2m1x2 %0, a;\n cvt.rn.f16x2.e2m1x2 %1, b;\n"
+      " cvt.rn.f16x2.e2m1x2 %2, c;\n cvt.rn.f16x2.e2m1x2 %3, d;\n}"
+      : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3])
+      : "r"(w));
+}
 // The 16 codes of 8 bytes times one scale.
 __device__ __forceinline__ void decode16(const uint2& w, float scale, float (&x)[16]) {
   const uint32_t part[2] = {w.x, w.y};
