@@ -123,6 +123,19 @@ class DeviceGuard {
   int back_ = -1;
 };
 
+// A kernel that continues the one launched just before it on the stream: always as a programmatic dependent launch, so that its
+// start overlaps that kernel's end (both wait for their predecessor in pdl_sync before they touch memory).
+template <typename... KArgs, typename... Args>
+inline cudaError_t launch_dependent(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, Args&&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid, cfg.blockDim = block, cfg.dynamicSmemBytes = smem, cfg.stream = stream;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at, cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, KArgs(std::forward<Args>(args))...);
+}
+
 struct DeviceInfo {
   int sms = 0;  // 0: not looked at yet
 };

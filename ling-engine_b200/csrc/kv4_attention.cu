@@ -13,8 +13,8 @@ using namespace d4;
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kPShift = 8.f;  // probabilities are carried times 2^8 in FP16: clear of its subnormals down to 2^-22
-constexpr int kStepKeys = 16;   // keys of one step of a warp: never crosses a page
 
+struct Join;
 struct AttnArgs {
   ling_b200_kv4 c;
   ling_b200_kv4_batch b;
@@ -23,9 +23,9 @@ struct AttnArgs {
   float scale;
   float* lse;
   int* err;
-  unsigned* tickets;
+  Join* joins;
   float* parts;
-  bool q_vec;  // four elements of q start on a boundary of four elements
+  bool q_vec;  // rows of q start on 16-byte boundaries
 };
 
 // ---------------------------------------------------------------------------------------------- few query rows
@@ -37,23 +37,86 @@ struct AttnArgs {
 //                 the same byte of two neighbouring keys, nibbles merged so that one cvt gives (key, key + 1) of a dim.  P
 //                 turns from an accumulator into a B fragment by movmatrix.  Values in FP16 are exact (E2M1 x E4M3 has 6
 //                 significant bits); q goes to FP16 times a power of two of its row, which loses nothing that a sum in fp32 keeps.
-//   loads         every warp streams its own 16-key steps by cp.async through a private ring of kStages; no block barriers
-//                 inside a context.
+//   loads         every warp streams its own steps (4.5 KB: 16, 32 or 64 keys) by cp.async through a private ring; the ring runs
+//                 on across the items of a CTA, and nothing inside an item waits for another warp.
 //   balance       the steps of all (sequence, kv head, row tile) items lie end to end and are cut into equal ranges, one per
-//                 CTA; an item that several CTAs share leaves partial results (O, m, l) and the last of them to arrive
-//                 adds them in order, so a result does not depend on the order of arrival.
-constexpr int kDecWarps = 8, kDecThreads = kDecWarps * 32, kDecRows = 8, kDecMaxCtas = 592;
+//                 worker: a CTA, whose warps take its steps in turn and add their results in shared memory, or (kSolo) a warp on
+//                 its own, which meets nobody.  An item that several workers share leaves partial results (O, m, l), which a
+//                 second kernel, launched dependent so that its start overlaps the first one's end, adds in order.
+constexpr int kDecRows = 8, kDecMaxCtas = 160;
+constexpr int kDecWarps = 8, kDecThreads = kDecWarps * 32, kDecMaxWorkers = kDecMaxCtas * kDecWarps;
+constexpr int kSoloItems = 74;
+constexpr float kLazy = 7.f;  // a score may exceed the running reference by this (log2) before the sums are scaled anew
 
-__host__ __device__ constexpr int dec_stages(int D) { return D == 256 ? 3 : D == 128 ? 5 : 8; }
-__host__ __device__ constexpr int dec_stage_bytes(int D) { return 18 * D; }  // 16 keys: codes 2 x 8 D, scales 2 x D
-__host__ __device__ constexpr int dec_smem(int D) { return kDecWarps * dec_stages(D) * dec_stage_bytes(D); }
+__host__ __device__ constexpr int dec_stages(int D) { return D == 256 ? 4 : 5; }
+__host__ __device__ constexpr int dec_sub(int D) { return 256 / D; }       // 16-key blocks of a step
+__host__ __device__ constexpr int dec_block_bytes(int D) { return 18 * D; }  // 16 keys: codes 2 x 8 D, scales 2 x D
+__host__ __device__ constexpr int dec_stage_bytes(int D) { return dec_sub(D) * dec_block_bytes(D); }
+__host__ __device__ constexpr int dec_q_stride(int D) { return 2 * D + 16; }  // bytes of a query row in shared memory (padded against bank conflicts)
+__host__ __device__ constexpr int dec_q_bytes(int D) { return kDecRows * dec_q_stride(D); }
+__host__ __device__ constexpr int dec_sum_bytes(int D) { return 32 * D; }   // a warp's O, raw: [D / 16][lane][4] floats
+__host__ __device__ constexpr int dec_smem(int D) {
+  return kDecWarps * dec_stages(D) * dec_stage_bytes(D) + kDecWarps / 2 * dec_sum_bytes(D) + dec_stages(D) * dec_q_bytes(D);
+}
 __host__ __device__ constexpr size_t dec_part_floats(int D) { return size_t(kDecRows) * D + 2 * kDecRows; }
 
-template <int N>
-__device__ __forceinline__ void cp_async(void* dst, const void* src) {
-  const uint32_t a = static_cast<uint32_t>(__cvta_generic_to_shared(dst));
-  if constexpr (N == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(a), "l"(src) : "memory");
-  else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(a), "l"(src), "n"(N) : "memory");
+// An item that goes on behind the CTA it starts in: what the join needs of it.  parts = 0: none.
+struct Join {
+  int parts, row0, rows, h, tile, pad[3];
+};
+
+// N bytes from src + SRC to the shared address dst + DST (the offsets ride in the instruction).
+template <int N, int DST, int SRC>
+__device__ __forceinline__ void cp_async(uint32_t dst, const void* src) {
+  if constexpr (N == 16) asm volatile("cp.async.cg.shared.global [%0 + %2], [%1 + %3], 16;" ::"r"(dst), "l"(src), "n"(DST), "n"(SRC) : "memory");
+  else asm volatile("cp.async.ca.shared.global [%0 + %2], [%1 + %3], %4;" ::"r"(dst), "l"(src), "n"(DST), "n"(SRC), "n"(N) : "memory");
+}
+// One 16-key block into a stage, by whole 512-byte lines of the cache: k, v and sc are the block's bytes from this lane's 16 (its
+// share of the scales) on.  Where a line lands is arranged so that the fragments are read without bank conflicts:
+//   K  key k, 16-byte chunk c:  D = 256: k * 128 + (c ^ 4 (k & 1)) * 16;  else as in the cache
+//   V  D = 256: key k, chunk c: k * 128 + (c ^ 2 t) * 16;  else the keys 2t + (j & 1) + 8 (j >> 1) in the order (j, t), D = 128 with chunk c
+//      at c ^ 2 (t >> 1)
+struct BlockDst {
+  uint32_t k, v, v2, sc;  // offsets of this lane in a stage (v2: V's second and fourth line, D = 256)
+};
+template <int D>
+__device__ __forceinline__ BlockDst block_dst(int lane) {
+  BlockDst d;
+  const int r = lane >> 3, c = lane & 7, r4 = lane >> 2, c4 = lane & 3, r2 = lane >> 1, c2 = lane & 1;
+  if constexpr (D == 256) {
+    d.k = r * 128 + ((c ^ (r & 1) * 4) * 16);
+    d.v = r * 128 + ((c ^ (r >> 1) * 2) * 16), d.v2 = r * 128 + ((c ^ (4 + (r >> 1) * 2)) * 16);
+  } else if constexpr (D == 128) {
+    d.k = lane * 16;
+    d.v = (r4 & 1) * 256 + (r4 >> 1) * 64 + ((c4 ^ (r4 >> 2) * 2) * 16), d.v2 = d.v;
+  } else {
+    d.k = lane * 16;
+    d.v = ((r2 >> 3) * 2 + (r2 & 1)) * 128 + (r2 >> 1 & 3) * 32 + c2 * 16, d.v2 = d.v;
+  }
+  d.sc = lane * (D / 16);
+  return d;
+}
+template <int D>
+__device__ __forceinline__ void cp_block(uint32_t stage, const BlockDst& d, const uint8_t* k, const uint8_t* v, const uint8_t* sc) {
+  cp_async<16, 0, 0>(stage + d.k, k);
+  if constexpr (D >= 128) cp_async<16, 512, 512>(stage + d.k, k);
+  if constexpr (D == 256) cp_async<16, 1024, 1024>(stage + d.k, k), cp_async<16, 1536, 1536>(stage + d.k, k);
+  cp_async<16, 8 * D, 0>(stage + d.v, v);
+  if constexpr (D >= 128) cp_async<16, 8 * D + 512, 512>(stage + d.v2, v);
+  if constexpr (D == 256) cp_async<16, 8 * D + 1024, 1024>(stage + d.v, v), cp_async<16, 8 * D + 1536, 1536>(stage + d.v2, v);
+  cp_async<D / 16, 16 * D, 0>(stage + d.sc, sc);
+}
+// Where this thread (g, t) finds piece p of key half * 8 + g, and its dims of V's key 2t + (j & 1) + 8 (j >> 1).
+template <int D>
+__device__ __forceinline__ int k_offset(int g, int t, int half, int p) {
+  if constexpr (D == 256) return (half * 8 + g) * 128 + (((p * 4 + t) ^ (g & 1) * 4) * 16);
+  return (half * 8 + g) * (D / 2) + t * (D / 8);
+}
+template <int D>
+__device__ __forceinline__ int v_offset(int g, int t, int j) {
+  if constexpr (D == 256) return (2 * t + (j & 1) + (j >> 1) * 8) * 128 + ((g ^ 2 * t) * 16);
+  if constexpr (D == 128) return (j * 4 + t) * 64 + (((g >> 1) ^ (t >> 1) * 2) * 16) + (g & 1) * 8;
+  return j * 128 + t * 32 + g * 4;
 }
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -61,13 +124,13 @@ __device__ __forceinline__ void cp_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 __device__ __forceinline__ void mma_16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ uint32_t movmatrix(uint32_t v) {
   uint32_t r;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
   return r;
 }
 __device__ __forceinline__ uint32_t h2(float lo, float hi) {
@@ -83,6 +146,9 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// What a partial result (reference m, sum l) counts for under the common reference: one without a visible key has l = 0, one whose
+// scores were all NaN has l = NaN and no m.
+__device__ __forceinline__ float part_weight(float m, float l, float common) { return m == -INFINITY ? (l == 0.f ? 0.f : 1.f) : ex2(m - common); }
 // B bytes of shared memory as 32-bit words.
 template <int B>
 __device__ __forceinline__ void lds(const uint8_t* p, uint32_t (&w)[B / 4]) {
@@ -97,105 +163,230 @@ __device__ __forceinline__ void lds(const uint8_t* p, uint32_t (&w)[B / 4]) {
   }
 }
 
-// What of the work lies where: an item is (sequence, kv head, tile of kDecRows query rows), `steps` 16-key steps long.
-struct Item {
-  int s, h, tile, steps;
-  Kv4Seq sq;
-};
-
+// Writes quad `quad` of an item's result: of the raw order [D / 16][lane][4], entry (i, lane) holds dims 2 i and 2 i + 1 of the
+// lane's D / 8 dims for query rows 2t and 2t + 1, as (row 2t, row 2t+1) of the first, then of the second dim.
 template <typename T, int D>
+__device__ __forceinline__ void store_quad(const AttnArgs& a, int row0, int n, int h, int tile, int quad, const float4& acc, const float (&mm)[2], const float (&ll)[2]) {
+  const int G = a.q_heads / a.c.kv_heads, lane = quad % 32, t = lane & 3, d = lane / 4 * (D / 8) + quad / 32 * 2;
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const int f = tile * kDecRows + 2 * t + j;
+    if (f >= n * G) continue;
+    const int row = row0 + f / G, head = h * G + f % G;
+    const bool empty = mm[j] == -INFINITY && ll[j] == 0.f;
+    const float scale = empty ? 0.f : a.c.v_scale / ll[j];
+    T* to = static_cast<T*>(a.out.p) + row * a.out.row + head * a.out.head + d;
+    to[0] = from_f32<T>(empty ? 0.f : (j ? acc.y : acc.x) * scale);
+    to[1] = from_f32<T>(empty ? 0.f : (j ? acc.w : acc.z) * scale);
+    if (a.lse && quad < 4) a.lse[size_t(row) * a.q_heads + head] = empty ? -INFINITY : (mm[j] + log2f(ll[j]) - kPShift) * kLn2;
+  }
+}
+
+template <typename T, int D, bool kSolo>
 __global__ void __launch_bounds__(kDecThreads, 1) kv4_decode_kernel(AttnArgs a) {
   pdl_sync();  // first statement: see common.cuh
-  constexpr int S = dec_stages(D), KP = D == 256 ? 2 : 1, KB = D == 64 ? 8 : 16, VB = D / 16, SB = D / 16;
-  constexpr int kK = 2 * KP * KB * 32, kV = 4 * VB * 32;  // bytes of a stage's K and V codes
-  static_assert(kK == 8 * D && kV == 8 * D, "a stage holds 16 keys");
+  constexpr int S = dec_stages(D), U = dec_sub(D), kKeys = 16 * U, kHalf = kDecWarps / 2;
+  constexpr int KP = D == 256 ? 2 : 1, KB = D == 64 ? 8 : 16, VB = D / 16, SB = D / 16;
+  constexpr int kK = 8 * D, kV = 8 * D;  // bytes of a block's K and V codes
+  constexpr int kStride = kSolo ? 1 : kDecWarps, kMinSteps = kSolo ? 4 : kDecWarps;
   extern __shared__ __align__(16) uint8_t smem[];
-  __shared__ long long first[LING_B200_KV4_MAX_SEQS + 1];  // steps of the sequences before s
+  __shared__ int first[LING_B200_KV4_MAX_SEQS + 1], steps_of[LING_B200_KV4_MAX_SEQS];  // steps of the sequences before s; of an item of s
   __shared__ float ml[kDecWarps][2][kDecRows];
-  __shared__ unsigned last;
+  __shared__ int quota_sh;    // steps of a worker
+  __shared__ bool round_sh;   // whether an item takes whole ranges
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-  const int G = a.q_heads / a.c.kv_heads, H = a.c.kv_heads, T_page = a.c.page_tokens;
+  const int workers = int(gridDim.x) * (kSolo ? kDecWarps : 1), me = kSolo ? int(blockIdx.x) * kDecWarps + warp : int(blockIdx.x);
+  const int turn = kSolo ? 0 : warp;  // the worker's steps this warp takes: turn, turn + kStride, ..
+  const int G = a.q_heads / a.c.kv_heads, H = a.c.kv_heads, lp = 31 - __clz(a.c.page_tokens);
+  uint8_t* ring = smem + warp * (S * dec_stage_bytes(D));
+  uint8_t* sums = smem + kDecWarps * S * dec_stage_bytes(D);
+  uint8_t* q_raw = sums + kHalf * dec_sum_bytes(D);
+  const uint32_t ring_u32 = static_cast<uint32_t>(__cvta_generic_to_shared(ring));
 
-  // ---- the sequences' steps, end to end
+  // ---- the items' steps, end to end, and a range of them for every worker (warp 0 counts)
   if (warp == 0) {
-    long long sum = 0;
+    int sum = 0, items = 0;
+    for (int s = lane; s < a.b.seqs; s += 32) {
+      const Kv4Seq q = kv4_seq(a.c, a.b, s);
+      if (!q.ok && blockIdx.x == 0) dev_fail(a.err, kDevBadBatch);
+      const int mine = q.ok && q.n > 0 ? (q.n * G + kDecRows - 1) / kDecRows * H : 0;
+      steps_of[s] = mine > 0 ? (q.pos + q.n + kKeys - 1) / kKeys : 0;
+      first[s + 1] = mine;
+      sum += mine * steps_of[s], items += mine;
+    }
+    sum = __reduce_add_sync(0xffffffffu, sum), items = __reduce_add_sync(0xffffffffu, items);
+    // no range is shorter than kMinSteps (a step for every warp of a CTA), unless the contexts themselves are
+    int quota = max(max((sum + workers - 1) / workers, min(kMinSteps, sum / max(items, 1))), 1);
+    const bool round = 4 * items <= workers;
+    if (round) {
+      // Several workers to an item: it takes whole ranges, so that no worker pays for two items (at most an eighth of them is lost to
+      // rounding).  The shortest range that suffices:
+      auto ranges = [&](int q) {
+        int n = 0;
+        for (int s = lane; s < a.b.seqs; s += 32) n += first[s + 1] * ((steps_of[s] + q - 1) / q);
+        return __reduce_add_sync(0xffffffffu, n);
+      };
+      int lo = quota - 1, hi = quota;
+      while (ranges(hi) > workers) lo = hi, hi *= 2;
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) / 2;
+        if (ranges(mid) > workers) lo = mid; else hi = mid;
+      }
+      quota = hi;
+    }
+    sum = 0;
     for (int s0 = 0; s0 < a.b.seqs; s0 += 32) {
       const int s = s0 + lane;
-      long long n = 0;
-      if (s < a.b.seqs) {
-        const Kv4Seq q = kv4_seq(a.c, a.b, s);
-        if (!q.ok && blockIdx.x == 0) dev_fail(a.err, kDevBadBatch);
-        if (q.ok && q.n > 0) n = (long long)((q.n * G + kDecRows - 1) / kDecRows) * H * ((q.pos + q.n + kStepKeys - 1) / kStepKeys);
-      }
+      int n = s < a.b.seqs ? first[s + 1] * (round ? (steps_of[s] + quota - 1) / quota * quota : steps_of[s]) : 0;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
-        const long long v = __shfl_up_sync(0xffffffffu, n, o);
+        const int v = __shfl_up_sync(0xffffffffu, n, o);
         if (lane >= o) n += v;
       }
       if (s < a.b.seqs) first[s + 1] = sum + n;
       sum += __shfl_sync(0xffffffffu, n, 31);
     }
-    if (lane == 0) first[0] = 0;
+    if (lane == 0) first[0] = 0, quota_sh = quota, round_sh = round;
   }
   __syncthreads();
-  const long long total = first[a.b.seqs];
-  const long long quota = (total + gridDim.x - 1) / gridDim.x;
-  long long at = quota * blockIdx.x;
-  const long long end = min(total, at + quota);
+  const int total = first[a.b.seqs], quota = quota_sh;
+  const bool round = round_sh;
+  const int begin = min(total, quota * me), end = min(total, begin + quota);
+  if (kSolo ? lane == 0 : tid == 0) a.joins[me].parts = 0;
+  if (begin >= end) return;
 
-  uint8_t* ring = smem + warp * (S * dec_stage_bytes(D));
-  while (at < end) {
-    // ---- the item that step `at` belongs to
-    int lo = 0, hi = a.b.seqs;  // first[lo] <= at < first[hi]
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) / 2;
-      if (first[mid] <= at) lo = mid; else hi = mid;
+  // The part of an item that starts at step `at` of this worker's range: first[seq] <= at < first[seq + 1].
+  struct Part {
+    Kv4Seq sq;
+    int keys, steps, step0, step1, next, h, tile, mine;  // mine: this warp's steps, step0 + turn and on by kStride
+  };
+  auto part_at = [&](int at) {
+    int seq = 0, hi = a.b.seqs;
+    while (hi - seq > 1) {
+      const int mid = (seq + hi) / 2;
+      if (first[mid] <= at) seq = mid; else hi = mid;
     }
-    Item it;
-    it.s = lo;
-    it.sq = kv4_seq(a.c, a.b, lo);
-    const int keys = it.sq.pos + it.sq.n, tiles = (it.sq.n * G + kDecRows - 1) / kDecRows;
-    it.steps = (keys + kStepKeys - 1) / kStepKeys;
-    const long long off = at - first[lo];
-    const int which = int(off / it.steps), step0 = int(off % it.steps);
-    it.h = which / tiles, it.tile = which % tiles;
-    const int step1 = int(min((long long)it.steps, step0 + (end - at)));
-    const long long item_first = at - step0;  // the item's steps are [item_first, item_first + steps)
+    Part p;
+    p.sq = kv4_seq(a.c, a.b, seq);
+    p.keys = p.sq.pos + p.sq.n;
+    p.steps = steps_of[seq];
+    const int len = round ? (p.steps + quota - 1) / quota * quota : p.steps;
+    const int tiles = (p.sq.n * G + kDecRows - 1) / kDecRows, which = (at - first[seq]) / len;
+    p.step0 = (at - first[seq]) - which * len;
+    p.step1 = min(p.steps, p.step0 + (end - at));
+    p.next = round ? end : at + (p.step1 - p.step0);
+    p.h = which / tiles, p.tile = which - p.h * tiles;
+    p.mine = max(0, (p.step1 - p.step0 - turn + kStride - 1) / kStride);
+    return p;
+  };
 
-    // ---- Q^T as B fragments: column g is query row f = tile * 8 + g, (row f / G, head f % G)
+  // ---- the loading side: runs S - 1 steps ahead of the computing side, across items
+  const BlockDst dst = block_dst<D>(lane);
+  const uint8_t* k_lane = a.c.k + lane * 16;
+  const uint8_t* v_lane = a.c.v + lane * 16;
+  const uint8_t* s_lane = (lane < 16 ? a.c.k_scales : a.c.v_scales) + (lane & 15) * SB;
+  int in_at = begin, in_part = 0;             // the next item part to load from, and its number among the worker's
+  int in_n = 0, in_mine = 0, in_pos = 0, in_keys = 0, in_h = 0;  // of the current one: this warp's steps, first position, ..
+  const int* in_table = nullptr;
+  int put = 0;          // the ring's next stage to fill
+  uint32_t block_of = 0, block_ok = 0;  // of the current 32 blocks: this lane's, among the cache's blocks of 16 tokens; whether the pages are ones
+  uint32_t good = 0;    // of the steps on their way, U bits each, youngest lowest: whether the blocks' pages are ones
+  auto issue = [&]() {
+    while (in_n == in_mine && in_at < end) {
+      const Part p = part_at(in_at);
+      in_at = p.next;
+      in_n = 0, in_mine = p.mine, in_pos = (p.step0 + turn) * kKeys, in_keys = p.keys, in_h = p.h;
+      in_table = a.c.tables + size_t(p.sq.slot) * a.c.max_pages;
+      // the query rows, row f = tile * 8 + r being (row f / G, head f % G): into shared memory as they are, or (kSolo) on their way to L2
+      if (kSolo || warp == 0) {
+        uint8_t* to = q_raw + in_part % S * dec_q_bytes(D);
+        for (int i = lane; i < kDecRows * (D / 8); i += 32) {
+          const int r = i / (D / 8), f = p.tile * kDecRows + r;
+          if (f >= p.sq.n * G) break;
+          const T* src = static_cast<const T*>(a.q.p) + (p.sq.row0 + f / G) * a.q.row + (p.h * G + f % G) * a.q.head + i % (D / 8) * 8;
+          uint8_t* dst = to + r * dec_q_stride(D) + i % (D / 8) * 16;
+          if constexpr (kSolo) {
+            asm volatile("prefetch.global.L2 [%0];" ::"l"(src));
+          } else if (a.q_vec) {
+            cp_async<16, 0, 0>(static_cast<uint32_t>(__cvta_generic_to_shared(dst)), src);
+          } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) reinterpret_cast<T*>(dst)[j] = src[j];
+          }
+        }
+      }
+      ++in_part;
+    }
+    if (in_n < in_mine) {
+      if ((in_n * U & 31) == 0) {  // the next 32 blocks: a lane looks one up
+        const int pos = in_pos + (in_n + lane / U) * (kStride * kKeys) + lane % U * 16;
+        const bool there = in_n + lane / U < in_mine && pos < in_keys;
+        const int page = there ? in_table[pos >> lp] : 0;
+        const bool ok = page >= 1 && page <= a.c.pages;
+        if (there && !ok) dev_fail(a.err, kDevBadPage);
+        block_ok = __ballot_sync(0xffffffffu, ok);  // the others are masked later; the reserved page stands in
+        block_of = ((uint32_t(ok ? page : 0) * H + in_h) << (lp - 4)) + ((pos & ((1 << lp) - 1)) >> 4);
+      }
+      uint32_t st = ring_u32 + put * dec_stage_bytes(D);
+      put = put + 1 == S ? 0 : put + 1;
+      good = good << U | (block_ok >> (in_n * U & 31) & ((1u << U) - 1u));
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const uint32_t block = __shfl_sync(0xffffffffu, block_of, (in_n * U + u) & 31);
+        cp_block<D>(st, dst, k_lane + size_t(block) * (8 * D), v_lane + size_t(block) * (8 * D), s_lane + size_t(block) * D);
+        st += dec_block_bytes(D);
+      }
+      ++in_n;
+    } else {
+      good <<= U;
+    }
+    cp_commit();
+  };
+#pragma unroll
+  for (int n = 0; n < S - 1; ++n) issue();
+
+  // ---- the computing side, item part by item part
+  int stage = 0;
+  for (int at = begin, number = 0; at < end; ++number) {
+    const Part p = part_at(at);
+    const int step0 = p.step0, step1 = p.step1, steps = p.steps, keys = p.keys, tile = p.tile, h = p.h, mine = p.mine;
+    const Kv4Seq sq = p.sq;
+    if constexpr (!kSolo) {
+      cp_wait<S - 2>();  // warp 0: the query rows travel with its first step of the part
+      __syncthreads();
+    }
+
+    // Q^T as B fragments in FP16 (column g is query row tile * 8 + g), each row times 2^(8 - exponent of its largest value): FP16
+    // keeps 2^-25 of an element whose row reaches 2^8.  A row with a value that is not finite becomes NaN, as its softmax would.
     uint32_t qb[D / 16][2];
     float inv;
     {
-      const int f = it.tile * kDecRows + g;
-      const bool real = f < it.sq.n * G;
-      const T* src = static_cast<const T*>(a.q.p) + (it.sq.row0 + (real ? f / G : 0)) * a.q.row + (it.h * G + (real ? f % G : 0)) * a.q.head;
-      float top = 0.f;
+      const int q_f = tile * kDecRows + g;
+      const bool real = q_f < sq.n * G;
+      const uint8_t* row = q_raw + number % S * dec_q_bytes(D) + g * dec_q_stride(D);
+      if constexpr (kSolo) row = reinterpret_cast<const uint8_t*>(static_cast<const T*>(a.q.p) + (sq.row0 + (real ? q_f / G : 0)) * a.q.row + (h * G + (real ? q_f % G : 0)) * a.q.head);
+      uint32_t top2 = 0;  // largest magnitudes of the pairs' halves: the bits of values of one sign order as integers, NaN highest
 #pragma unroll
       for (int kk = 0; kk < D / 16; ++kk) {
-        const int d = D == 256 ? (kk / 8) * 128 + t * 32 + (kk % 8) * 4 : t * (D / 4) + kk * 4;
-        T e[4];
-        if (a.q_vec) {
-          *reinterpret_cast<uint2*>(e) = *reinterpret_cast<const uint2*>(src + d);
+        const uint8_t* four = row + 2 * (D == 256 ? (kk / 8) * 128 + t * 32 + (kk % 8) * 4 : t * (D / 4) + kk * 4);
+        uint2 w;
+        if (!kSolo || a.q_vec) {
+          w = *reinterpret_cast<const uint2*>(four);
         } else {
-#pragma unroll
-          for (int j = 0; j < 4; ++j) e[j] = src[d + j];
+          const uint16_t* e = reinterpret_cast<const uint16_t*>(four);
+          w = make_uint2(e[0] | uint32_t(e[1]) << 16, e[2] | uint32_t(e[3]) << 16);
         }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float v = fabsf(to_f32<T>(e[j]));
-          top = v > top || v != v ? v : top;  // a NaN stays
-        }
-        qb[kk][0] = reinterpret_cast<uint32_t*>(e)[0], qb[kk][1] = reinterpret_cast<uint32_t*>(e)[1];
+        qb[kk][0] = w.x, qb[kk][1] = w.y;
+        top2 = __vmaxu2(top2, __vmaxu2(w.x & 0x7fff7fffu, w.y & 0x7fff7fffu));
       }
 #pragma unroll
-      for (int o = 1; o < 4; o <<= 1) {
-        const float v = __shfl_xor_sync(0xffffffffu, top, o);
-        top = v > top || v != v ? v : top;
-      }
-      // the row times 2^(8 - exponent of its largest value): FP16 keeps 2^-25 of an element whose row reaches 2^8
+      for (int o = 1; o < 4; o <<= 1) top2 = __vmaxu2(top2, __shfl_xor_sync(0xffffffffu, top2, o));
+      const uint16_t top_bits = uint16_t(max(top2 & 0xffffu, top2 >> 16));
+      const float top = to_f32<T>(*reinterpret_cast<const T*>(&top_bits));
       const int ex = int(__float_as_uint(top) >> 23 & 255u), field = min(max(262 - ex, 2), 252);
-      const float mul = top == 0.f ? 1.f : top < INFINITY ? __uint_as_float(uint32_t(field) << 23) : NAN;
-      inv = top > 0.f && top < INFINITY ? __uint_as_float(uint32_t(254 - field) << 23) : 1.f;
+      const float sign = a.scale < 0.f ? -1.f : 1.f;  // the queries carry the scale's sign
+      const float mul = sign * (top == 0.f ? 1.f : top < INFINITY ? __uint_as_float(uint32_t(field) << 23) : NAN);
+      inv = top > 0.f && top < INFINITY && real ? __uint_as_float(uint32_t(254 - field) << 23) : 1.f;
 #pragma unroll
       for (int kk = 0; kk < D / 16; ++kk)
 #pragma unroll
@@ -205,148 +396,127 @@ __global__ void __launch_bounds__(kDecThreads, 1) kv4_decode_kernel(AttnArgs a) 
         }
     }
     // this thread's score columns are query rows 2t and 2t + 1
-    const float to_log2 = a.scale * a.c.k_scale * kLog2e;
     float coef[2];
     uint32_t see[2];  // in-flight rows each sees, as a mask or (no masks) their number
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-      coef[j] = to_log2 * __shfl_sync(0xffffffffu, inv, (2 * t + j) * 4);
-      const int f = it.tile * kDecRows + 2 * t + j, i = f / G;
-      see[j] = i >= it.sq.n ? 0u : a.b.anc ? a.b.anc[it.sq.row0 + i] : uint32_t(i + 1);
+      coef[j] = fabsf(a.scale) * a.c.k_scale * kLog2e * __shfl_sync(0xffffffffu, inv, (2 * t + j) * 4);
+      const int i = (tile * kDecRows + 2 * t + j) / G;
+      see[j] = i >= sq.n ? 0u : a.b.anc ? a.b.anc[sq.row0 + i] : uint32_t(i + 1);
     }
 
     float o[D / 16][4] = {}, m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-
-    // ---- this warp's steps: step0 + warp, step0 + warp + 8, ...
-    const int* table = a.c.tables + size_t(it.sq.slot) * a.c.max_pages;
-    const int mine = (step1 - step0 - warp + kDecWarps - 1) / kDecWarps;
-    int page_batch = 0;   // this lane's page of the current 32 steps
-    uint32_t good = 0;    // of the steps on their way, youngest in bit 0: whether the page is one
-    auto issue = [&](int n) {
-      if (n < mine) {
-        if ((n & 31) == 0) {
-          const int st = step0 + warp + (n + lane) * kDecWarps;
-          page_batch = n + lane < mine ? table[st * kStepKeys / T_page] : 0;
-        }
-        int page = __shfl_sync(0xffffffffu, page_batch, n & 31);
-        const bool ok = page >= 1 && page <= a.c.pages;
-        if (!ok) {
-          if (lane == 0) dev_fail(a.err, kDevBadPage);
-          page = 0;  // the reserved page: its keys are masked
-        }
-        good = good << 1 | (ok ? 1u : 0u);
-        const int pos = (step0 + warp + n * kDecWarps) * kStepKeys;
-        const size_t vec = kv4_vector(a.c, page, it.h, pos % T_page);
-        uint8_t* st = ring + (n % S) * dec_stage_bytes(D);
-        const uint8_t* k = a.c.k + vec * (D / 2) + g * (D / 2) + t * KB;
-#pragma unroll
-        for (int half = 0; half < 2; ++half)
-#pragma unroll
-          for (int p = 0; p < KP; ++p) cp_async<KB>(st + ((half * KP + p) * 32 + lane) * KB, k + half * 8 * (D / 2) + p * 64);
-        const uint8_t* v = a.c.v + vec * (D / 2) + 2 * t * (D / 2) + g * VB;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) cp_async<VB>(st + kK + (j * 32 + lane) * VB, v + (j / 2 * 8 + j % 2) * (D / 2));
-        const uint8_t* sc = (lane < 16 ? a.c.k_scales : a.c.v_scales) + vec * SB + (lane & 15) * SB;
-        cp_async<SB>(st + kK + kV + lane * SB, sc);
-      } else {
-        good <<= 1;
-      }
-      cp_commit();
-    };
-#pragma unroll
-    for (int n = 0; n < S - 1; ++n) issue(n);
     for (int n = 0; n < mine; ++n) {
       cp_wait<S - 2>();
-      __syncwarp();  // step n has landed, for all lanes; all lanes are done with step n - 1, whose stage is next
-      issue(n + S - 1);
-      const uint8_t* st = ring + (n % S) * dec_stage_bytes(D);
-      const uint8_t* ks = st + kK + kV;
-      const uint8_t* vs = ks + D;
-      const int pos0 = (step0 + warp + n * kDecWarps) * kStepKeys;
-      const bool masked = !(good >> (S - 1) & 1u) || pos0 + kStepKeys > it.sq.pos;
+      __syncwarp();  // the step has landed, for all lanes; all lanes are done with the one before, whose stage is next
+      issue();
+      const uint8_t* st = ring + stage * dec_stage_bytes(D);
+      stage = stage + 1 == S ? 0 : stage + 1;
+      const int pos0 = (step0 + turn + n * kStride) * kKeys;
+      const uint32_t ok_bits = good >> (S - 1) * U & ((1u << U) - 1u);  // block u in bit u
+      const bool masked = ok_bits != (1u << U) - 1u || pos0 + kKeys > sq.pos;
 
       // scores
-      float s[4] = {0.f, 0.f, 0.f, 0.f}, s2[4] = {0.f, 0.f, 0.f, 0.f};
+      float s[U][4];
 #pragma unroll
-      for (int p = 0; p < KP; ++p) {
-        uint32_t w[2][KB / 4], sc[2][KB / 8];  // of keys g and g + 8: codes, scales by group as half2
+      for (int u = 0; u < U; ++u) {
+        const uint8_t* kc = st + u * dec_block_bytes(D);
+        const uint8_t* ks = kc + kK + kV;
+        float s2[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          lds<KB>(st + ((half * KP + p) * 32 + lane) * KB, w[half]);
-          const uint8_t* at_s = ks + (half * 8 + g) * SB + (KB == 16 ? p * 8 + t * 2 : t);
-          const uint32_t pair = KB == 16 ? *reinterpret_cast<const uint16_t*>(at_s) : *at_s;
-          const uint32_t h = e4m3x2_to_h2(uint16_t(pair));
-          sc[half][0] = __byte_perm(h, h, 0x1010);
-          if constexpr (KB == 16) sc[half][1] = __byte_perm(h, h, 0x3232);
-        }
+        for (int j = 0; j < 4; ++j) s[u][j] = 0.f;
 #pragma unroll
-        for (int i = 0; i < KB / 4; ++i) {  // word i: 8 codes, two MMAs
-          uint32_t c[2][4];
+        for (int p = 0; p < KP; ++p) {
+          uint32_t w[2][KB / 4], sc[2][KB / 8];  // of keys g and g + 8: codes, scales by group as half2
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
-            e2m1x8_to_h2(w[half][i], c[half]);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) c[half][j] = h2_mul(c[half][j], sc[half][i / 2]);
+            lds<KB>(kc + k_offset<D>(g, t, half, p), w[half]);
+            const uint8_t* at_s = ks + (half * 8 + g) * SB + (KB == 16 ? p * 8 + t * 2 : t);
+            const uint32_t pair = KB == 16 ? *reinterpret_cast<const uint16_t*>(at_s) : *at_s;
+            const uint32_t h = e4m3x2_to_h2(uint16_t(pair));
+            sc[half][0] = __byte_perm(h, h, 0x1010);
+            if constexpr (KB == 16) sc[half][1] = __byte_perm(h, h, 0x3232);
           }
-          const int kk = p * (KB / 2) + i * 2;
-          mma_16816(s, c[0][0], c[1][0], c[0][1], c[1][1], qb[kk][0], qb[kk][1]);
-          mma_16816(s2, c[0][2], c[1][2], c[0][3], c[1][3], qb[kk + 1][0], qb[kk + 1][1]);
+#pragma unroll
+          for (int i = 0; i < KB / 4; ++i) {  // word i: 8 codes, two MMAs
+            uint32_t c[2][4];
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+              e2m1x8_to_h2(w[half][i], c[half]);
+#pragma unroll
+              for (int j = 0; j < 4; ++j) c[half][j] = h2_mul(c[half][j], sc[half][i / 2]);
+            }
+            const int kk = p * (KB / 2) + i * 2;
+            mma_16816(s[u], c[0][0], c[1][0], c[0][1], c[1][1], qb[kk][0], qb[kk][1]);
+            mma_16816(U == 1 ? s2 : s[u], c[0][2], c[1][2], c[0][3], c[1][3], qb[kk + 1][0], qb[kk + 1][1]);  // (two chains where one block is all there is)
+          }
+        }
+        if constexpr (U == 1) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) s[u][j] += s2[j];
         }
       }
-#pragma unroll
-      for (int j = 0; j < 4; ++j) s[j] = (s[j] + s2[j]) * coef[j & 1];
 
       // V's scales: of this thread's key pairs (2t, 2t+1) and (2t+8, 2t+9), per group of its dims, as (key, key + 1)
       constexpr int VG = D == 256 ? 2 : 1;
-      uint32_t vsc[2][VG];
+      uint32_t vsc[U][2][VG], poison = 0;  // poison: of this thread's (block, key, row): a visible key whose V is NaN
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const uint8_t* at_s = vs + (2 * t + j * 8) * SB + (D == 256 ? g * 2 : D == 128 ? g : g / 2);
-        if constexpr (D == 256) {
-          const uint32_t x = *reinterpret_cast<const uint16_t*>(at_s), y = *reinterpret_cast<const uint16_t*>(at_s + SB);
-          vsc[j][0] = x & 0xffu | (y & 0xffu) << 8, vsc[j][1] = x >> 8 | y & 0xff00u;
-        } else {
-          vsc[j][0] = uint32_t(at_s[0]) | uint32_t(at_s[SB]) << 8;
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const uint8_t* at_s = st + u * dec_block_bytes(D) + kK + kV + D + (2 * t + j * 8) * SB + (D == 256 ? g * 2 : D == 128 ? g : g / 2);
+          if constexpr (D == 256) {
+            const uint32_t x = *reinterpret_cast<const uint16_t*>(at_s), y = *reinterpret_cast<const uint16_t*>(at_s + SB);
+            vsc[u][j][0] = __byte_perm(x, y, 0x0040) & 0xffffu, vsc[u][j][1] = __byte_perm(x, y, 0x0051) & 0xffffu;
+          } else {
+            vsc[u][j][0] = uint32_t(at_s[0]) | uint32_t(at_s[SB]) << 8;
+          }
         }
-      }
-      uint32_t poison = 0;  // of this thread's four (key, row): a visible key whose V is NaN
+      uint32_t vw[U][4][VB / 4];  // (asked for ahead of the softmax)
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) lds<VB>(st + u * dec_block_bytes(D) + kK + v_offset<D>(g, t, j), vw[u][j]);
       if (masked) {
         // A V vector that is NaN must reach exactly the rows that see it: its scale is taken as 0 and its probability as NaN.
-        uint32_t nan = 0;  // keys of this step
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
+        for (int u = 0; u < U; ++u) {
+          uint32_t nan = 0;  // keys of this block
 #pragma unroll
-          for (int v = 0; v < VG; ++v)
+          for (int j = 0; j < 2; ++j)
 #pragma unroll
-            for (int e = 0; e < 2; ++e)
-              if ((vsc[j][v] >> (8 * e) & 0x7fu) == 0x7fu) {
-                nan |= 1u << (2 * t + j * 8 + e);
-                vsc[j][v] &= e ? 0x00ffu : 0xff00u;
-              }
-        nan = __reduce_or_sync(0xffffffffu, nan);
-        const bool page_ok = good >> (S - 1) & 1u;
+            for (int v = 0; v < VG; ++v)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int key = g + (j >> 1) * 8, pos = pos0 + key, i = pos - it.sq.pos;
-          const uint32_t mask = see[j & 1];
-          const bool visible = page_ok && pos < keys && (i < 0 || (a.b.anc ? (mask >> i & 1u) : i < int(mask)));
-          if (!visible) s[j] = -INFINITY;
-          else poison |= (nan >> key & 1u) << j;
+              for (int e = 0; e < 2; ++e)
+                if ((vsc[u][j][v] >> (8 * e) & 0x7fu) == 0x7fu) {
+                  nan |= 1u << (2 * t + j * 8 + e);
+                  vsc[u][j][v] &= e ? 0x00ffu : 0xff00u;
+                }
+          nan = __reduce_or_sync(0xffffffffu, nan);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int key = g + (j >> 1) * 8, pos = pos0 + u * 16 + key, i = pos - sq.pos;
+            const uint32_t mask = see[j & 1];
+            const bool visible = (ok_bits >> u & 1u) && pos < keys && (i < 0 || (a.b.anc ? (mask >> i & 1u) : i < int(mask)));
+            if (!visible) s[u][j] = -INFINITY;
+            else poison |= (nan >> key & 1u) << (u * 4 + j);
+          }
         }
       }
 
-      // running maximum and sum; rows are columns 2t, 2t + 1, keys lie across the lanes with the same t
-      float mx[2] = {fmaxf(s[0], s[2]), fmaxf(s[1], s[3])};
+      // Scores are s * coef, coef >= 0.  The sums are kept relative to a reference m of each row, not its maximum: as long as no score exceeds it by 2^kLazy,
+      // P (times 2^8) stays inside FP16 and nothing is exchanged or scaled.  Rows are columns 2t, 2t + 1; keys lie across the
+      // lanes with the same t.
+      float mx[2] = {fmaxf(s[0][0], s[0][2]), fmaxf(s[0][1], s[0][3])};
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-#pragma unroll
-        for (int x = 4; x < 32; x <<= 1) mx[j] = fmaxf(mx[j], __shfl_xor_sync(0xffffffffu, mx[j], x));
-        mx[j] = fmaxf(mx[j], m[j]);
-      }
-      if (__any_sync(0xffffffffu, mx[0] > m[0] || mx[1] > m[1])) {
+      for (int u = 1; u < U; ++u) mx[0] = fmaxf(mx[0], fmaxf(s[u][0], s[u][2])), mx[1] = fmaxf(mx[1], fmaxf(s[u][1], s[u][3]));
+      if (__any_sync(0xffffffffu, fmaf(mx[0], coef[0], -m[0]) > kLazy || fmaf(mx[1], coef[1], -m[1]) > kLazy)) {
         float keep[2];
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
+#pragma unroll
+          for (int x = 4; x < 32; x <<= 1) mx[j] = fmaxf(mx[j], __shfl_xor_sync(0xffffffffu, mx[j], x));
+          mx[j] = fmaxf(mx[j] * coef[j], m[j]);
           keep[j] = m[j] == -INFINITY ? 0.f : ex2(m[j] - mx[j]);
           l[j] *= keep[j];
           m[j] = mx[j];
@@ -354,168 +524,210 @@ __global__ void __launch_bounds__(kDecThreads, 1) kv4_decode_kernel(AttnArgs a) 
 #pragma unroll
         for (int i = 0; i < D / 16; ++i) o[i][0] *= keep[0], o[i][2] *= keep[0], o[i][1] *= keep[1], o[i][3] *= keep[1];
       }
-      float p[4];
+      const float base[2] = {m[0] == -INFINITY ? 0.f : m[0] - kPShift, m[1] == -INFINITY ? 0.f : m[1] - kPShift};
 #pragma unroll
-      for (int j = 0; j < 4; ++j) p[j] = ex2(s[j] - (m[j & 1] == -INFINITY ? 0.f : m[j & 1] - kPShift));
-      l[0] += p[0] + p[2], l[1] += p[1] + p[3];
-      if (poison) {
+      for (int u = 0; u < U; ++u) {
+        float p[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) p[j] = poison >> j & 1u ? NAN : p[j];
-      }
-      const uint32_t b0 = movmatrix(h2(p[0], p[1])), b1 = movmatrix(h2(p[2], p[3]));
-
-      // values
-      uint32_t v[4][VB / 4], vh[2][VG];
+        for (int j = 0; j < 4; ++j) p[j] = ex2(fmaf(s[u][j], coef[j & 1], -base[j & 1]));
+        l[0] += p[0] + p[2], l[1] += p[1] + p[3];
+        if (poison) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) lds<VB>(st + kK + (j * 32 + lane) * VB, v[j]);
-#pragma unroll
-      for (int j = 0; j < 2; ++j)
-#pragma unroll
-        for (int x = 0; x < VG; ++x) vh[j][x] = e4m3x2_to_h2(uint16_t(vsc[j][x]));
-#pragma unroll
-      for (int i = 0; i < VB / 4; ++i) {  // word i: 8 dims, four MMAs' rows g (even dims) and g + 8 (odd dims)
-        uint32_t even[2][4], odd[2][4];
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const uint32_t x = v[2 * j][i], y = v[2 * j + 1][i];
-          e2m1x8_to_h2(x & 0x0f0f0f0fu | (y & 0x0f0f0f0fu) << 4, even[j]);
-          e2m1x8_to_h2(x >> 4 & 0x0f0f0f0fu | y & 0xf0f0f0f0u, odd[j]);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const uint32_t f = vh[j][VG == 2 ? i / 2 : 0];
-            even[j][e] = h2_mul(even[j][e], f), odd[j][e] = h2_mul(odd[j][e], f);
-          }
+          for (int j = 0; j < 4; ++j) p[j] = poison >> (u * 4 + j) & 1u ? NAN : p[j];
         }
+        const uint32_t b0 = movmatrix(h2(p[0], p[1])), b1 = movmatrix(h2(p[2], p[3]));
+        uint32_t vh[2][VG];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) mma_16816(o[i * 4 + e], even[0][e], odd[0][e], even[1][e], odd[1][e], b0, b1);
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int x = 0; x < VG; ++x) vh[j][x] = e4m3x2_to_h2(uint16_t(vsc[u][j][x]));
+#pragma unroll
+        for (int i = 0; i < VB / 4; ++i) {  // word i: 8 dims, four MMAs' rows g (even dims) and g + 8 (odd dims)
+          uint32_t even[2][4], odd[2][4];
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const uint32_t x = vw[u][2 * j][i], y = vw[u][2 * j + 1][i];
+            e2m1x8_to_h2(x & 0x0f0f0f0fu | (y << 4 & 0xf0f0f0f0u), even[j]);
+            e2m1x8_to_h2(x >> 4 & 0x0f0f0f0fu | y & 0xf0f0f0f0u, odd[j]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const uint32_t f = vh[j][VG == 2 ? i / 2 : 0];
+              even[j][e] = h2_mul(even[j][e], f), odd[j][e] = h2_mul(odd[j][e], f);
+            }
+          }
+#pragma unroll
+          for (int e = 0; e < 4; ++e) mma_16816(o[i * 4 + e], even[0][e], odd[0][e], even[1][e], odd[1][e], b0, b1);
+        }
       }
     }
-    cp_wait<0>();
 
-    // ---- the warps' results meet in shared memory (each warp's own ring), raw: [D / 16][lane][4]
 #pragma unroll
     for (int j = 0; j < 2; ++j)
 #pragma unroll
       for (int x = 4; x < 32; x <<= 1) l[j] += __shfl_xor_sync(0xffffffffu, l[j], x);
-    __syncwarp();
-    float4* mine_o = reinterpret_cast<float4*>(ring);
+    const bool whole = step0 == 0 && step1 == steps;
+    const int first_of = (at - step0) / quota, last_of = (at - step0 + steps - 1) / quota;  // the workers that share the item
+    // A worker has at most two parts of shared items: of the one it opens with (slot 0), of one that goes on behind it (slot 1).
+    float* part = a.parts + (size_t(me) * 2 + (me == first_of ? 1 : 0)) * dec_part_floats(D);
+    const Join join{last_of - first_of + 1, sq.row0, sq.n, h, tile, {0, 0, 0}};
+    at = p.next;
+    if constexpr (kSolo) {
 #pragma unroll
-    for (int i = 0; i < D / 16; ++i) mine_o[i * 32 + lane] = make_float4(o[i][0], o[i][1], o[i][2], o[i][3]);
+      for (int i = 0; i < D / 16; ++i) {
+        const float4 acc = make_float4(o[i][0], o[i][1], o[i][2], o[i][3]);
+        if (whole) store_quad<T, D>(a, sq.row0, sq.n, h, tile, i * 32 + lane, acc, m, l);
+        else reinterpret_cast<float4*>(part)[i * 32 + lane] = acc;
+      }
+      if (!whole) {
+        float* pm = part + kDecRows * D;
+        if (lane < 4) pm[2 * lane] = m[0], pm[2 * lane + 1] = m[1], pm[kDecRows + 2 * lane] = l[0], pm[kDecRows + 2 * lane + 1] = l[1];
+        if (lane == 0 && me == first_of) a.joins[me] = join;
+      }
+      continue;
+    }
+
+    // ---- the warps' results meet: the upper half's in shared memory, added to the lower half's, those added by all threads
     if (lane < 4) ml[warp][0][2 * lane] = m[0], ml[warp][0][2 * lane + 1] = m[1], ml[warp][1][2 * lane] = l[0], ml[warp][1][2 * lane + 1] = l[1];
+    float4* mine_o = reinterpret_cast<float4*>(sums + warp % kHalf * dec_sum_bytes(D)) + lane;
+    if (warp >= kHalf) {
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i) mine_o[i * 32] = make_float4(o[i][0], o[i][1], o[i][2], o[i][3]);
+    }
     __syncthreads();
-    const bool whole = step0 == 0 && step1 == it.steps;
-    constexpr int kQuads = D / 16 * 32, kEach = (kQuads + kDecThreads - 1) / kDecThreads;
-    float4 acc[kEach];
-    float mm[2], ll[2];  // of this thread's rows 2t', 2t' + 1 (t' of the quad's lane: the same for all its quads)
+    float mm[2], ll[2], own[2], other[2];  // of rows 2t, 2t + 1: common reference and sum, weights of this warp and its partner
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-      const int row = 2 * t + j;
+      float mw[kDecWarps], lw[kDecWarps];
       mm[j] = -INFINITY, ll[j] = 0.f;
 #pragma unroll
-      for (int w = 0; w < kDecWarps; ++w) mm[j] = fmaxf(mm[j], ml[w][0][row]);
+      for (int w = 0; w < kDecWarps; ++w) mw[w] = ml[w][0][2 * t + j], lw[w] = ml[w][1][2 * t + j], mm[j] = fmaxf(mm[j], mw[w]);
+#pragma unroll
+      for (int w = 0; w < kDecWarps; ++w) ll[j] = fmaf(lw[w], part_weight(mw[w], lw[w], mm[j]), ll[j]);
+      own[j] = part_weight(m[j], l[j], mm[j]);
+      const int w = (warp + kHalf) % kDecWarps;
+      other[j] = part_weight(ml[w][0][2 * t + j], ml[w][1][2 * t + j], mm[j]);
     }
+    if (warp < kHalf) {
 #pragma unroll
-    for (int e = 0; e < kEach; ++e) acc[e] = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-    for (int w = 0; w < kDecWarps; ++w) {
-      float f[2];
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const float mw = ml[w][0][2 * t + j];
-        f[j] = mw == -INFINITY ? (ml[w][1][2 * t + j] == 0.f ? 0.f : 1.f) : ex2(mw - mm[j]);
-        ll[j] = fmaf(ml[w][1][2 * t + j], f[j], ll[j]);
-      }
-#pragma unroll
-      for (int e = 0; e < kEach; ++e) {
-        const int quad = tid + e * kDecThreads;
-        if (quad < kQuads) {
-          const float4 x = reinterpret_cast<const float4*>(smem + w * (S * dec_stage_bytes(D)))[quad];
-          acc[e].x = fmaf(x.x, f[0], acc[e].x), acc[e].y = fmaf(x.y, f[1], acc[e].y);
-          acc[e].z = fmaf(x.z, f[0], acc[e].z), acc[e].w = fmaf(x.w, f[1], acc[e].w);
-        }
+      for (int i = 0; i < D / 16; ++i) {
+        const float4 x = mine_o[i * 32];
+        mine_o[i * 32] = make_float4(fmaf(o[i][0], own[0], x.x * other[0]), fmaf(o[i][1], own[1], x.y * other[1]),
+                                     fmaf(o[i][2], own[0], x.z * other[0]), fmaf(o[i][3], own[1], x.w * other[1]));
       }
     }
-    bool write = whole;
+    __syncthreads();
+    constexpr int kQuads = D / 16 * 32;
+#pragma unroll
+    for (int quad = tid; quad < kQuads; quad += kDecThreads) {
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int w = 0; w < kHalf; ++w) {
+        const float4 x = reinterpret_cast<const float4*>(sums + w * dec_sum_bytes(D))[quad];
+        acc.x += x.x, acc.y += x.y, acc.z += x.z, acc.w += x.w;
+      }
+      if (whole) store_quad<T, D>(a, sq.row0, sq.n, h, tile, quad, acc, mm, ll);
+      else reinterpret_cast<float4*>(part)[quad] = acc;
+    }
     if (!whole) {
-      // ---- a part of the item: left for the last of its CTAs.  A CTA has at most two parts: of the item it opens with (slot
-      // 0) and of one that goes on behind it (slot 1), whose ticket is the CTA's own.
-      const int cta0 = int(item_first / quota), cta1 = int((item_first + it.steps - 1) / quota);
-      const bool head = int(blockIdx.x) == cta0;
-      float* part = a.parts + (size_t(blockIdx.x) * 2 + (head ? 1 : 0)) * dec_part_floats(D);
-#pragma unroll
-      for (int e = 0; e < kEach; ++e)
-        if (tid + e * kDecThreads < kQuads) reinterpret_cast<float4*>(part)[tid + e * kDecThreads] = acc[e];
       if (tid < 4) {
         float* pm = part + kDecRows * D;
         pm[2 * tid] = mm[0], pm[2 * tid + 1] = mm[1], pm[kDecRows + 2 * tid] = ll[0], pm[kDecRows + 2 * tid + 1] = ll[1];
       }
-      __threadfence();
-      __syncthreads();
-      if (tid == 0) last = atomicInc(&a.tickets[cta0], unsigned(cta1 - cta0)) == unsigned(cta1 - cta0) ? 1u : 0u;
-      __syncthreads();
-      write = last != 0;
-      if (write) {
-        __threadfence();
-        mm[0] = mm[1] = -INFINITY, ll[0] = ll[1] = 0.f;
-        for (int c = cta0; c <= cta1; ++c) {
-          const float* pm = a.parts + (size_t(c) * 2 + (c == cta0 ? 1 : 0)) * dec_part_floats(D) + kDecRows * D;
-#pragma unroll
-          for (int j = 0; j < 2; ++j) mm[j] = fmaxf(mm[j], __ldcg(pm + 2 * t + j));
-        }
-#pragma unroll
-        for (int e = 0; e < kEach; ++e) acc[e] = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-        for (int c = cta0; c <= cta1; ++c) {
-          const float* pp = a.parts + (size_t(c) * 2 + (c == cta0 ? 1 : 0)) * dec_part_floats(D);
-          const float* pm = pp + kDecRows * D;
-          float f[2];
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const float mw = __ldcg(pm + 2 * t + j), lw = __ldcg(pm + kDecRows + 2 * t + j);
-            f[j] = mw == -INFINITY ? (lw == 0.f ? 0.f : 1.f) : ex2(mw - mm[j]);
-            ll[j] = fmaf(lw, f[j], ll[j]);
-          }
-#pragma unroll
-          for (int e = 0; e < kEach; ++e) {
-            const int quad = tid + e * kDecThreads;
-            if (quad < kQuads) {
-              const float4 x = __ldcg(reinterpret_cast<const float4*>(pp) + quad);
-              acc[e].x = fmaf(x.x, f[0], acc[e].x), acc[e].y = fmaf(x.y, f[1], acc[e].y);
-              acc[e].z = fmaf(x.z, f[0], acc[e].z), acc[e].w = fmaf(x.w, f[1], acc[e].w);
-            }
-          }
-        }
-      }
+      if (tid == 0 && me == first_of) a.joins[me] = join;
     }
-    if (write) {
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const int f = it.tile * kDecRows + 2 * t + j;
-        if (f >= it.sq.n * G) continue;
-        const int row = it.sq.row0 + f / G, head = it.h * G + f % G;
-        const bool empty = mm[j] == -INFINITY && ll[j] == 0.f;
-        const float scale = empty ? 0.f : a.c.v_scale / ll[j];
-        T* to = static_cast<T*>(a.out.p) + row * a.out.row + head * a.out.head;
-#pragma unroll
-        for (int e = 0; e < kEach; ++e) {
-          const int quad = tid + e * kDecThreads;
-          if (quad < kQuads) {
-            const int d = (quad % 32 / 4) * (D / 8) + quad / 32 * 2;  // raw quad (i, lane): dims 2 i, 2 i + 1 of lane's chunk
-            to[d] = from_f32<T>(empty ? 0.f : (j ? acc[e].y : acc[e].x) * scale);
-            to[d + 1] = from_f32<T>(empty ? 0.f : (j ? acc[e].w : acc[e].z) * scale);
-          }
-        }
-        if (a.lse && tid < 4) a.lse[size_t(row) * a.q_heads + head] = empty ? -INFINITY : (mm[j] + log2f(ll[j]) - kPShift) * kLn2;
-      }
-    }
-    __syncthreads();  // the shared results are read: the rings are free
-    at += step1 - step0;
+    // (the next part's opening barrier keeps its results off these sums)
   }
+  cp_wait<0>();
+}
+
+// The partial results of the items that workers of the decode kernel shared: block (w, piece) adds kJoinThreads / kSplit quads of
+// the item that starts with worker w and goes on behind it, kSplit threads a quad.
+constexpr int kJoinThreads = 256, kJoinParts = 160;  // parts whose weights are held at a time
+template <typename T, int D, int kSplit>
+__global__ void __launch_bounds__(kJoinThreads) kv4_join_kernel(AttnArgs a) {
+  pdl_sync();  // first statement: see common.cuh
+  constexpr int kEach = kJoinThreads / kSplit, kQuads = 2 * D;
+  __shared__ float pml[kJoinParts][2][kDecRows], red[2][kJoinThreads / 32][kDecRows];
+  __shared__ float4 sums[kSplit][kEach];
+  const int w0 = blockIdx.x, tid = threadIdx.x, lane = tid & 31, t = lane & 3, row = tid & 7, group = tid / kEach, quad = blockIdx.y * kEach + tid % kEach;
+  const Join join = a.joins[w0];
+  if (join.parts == 0) return;
+  const int n = join.parts;
+  auto part_of = [&](int i) { return a.parts + (size_t(w0 + i) * 2 + (i == 0 ? 1 : 0)) * dec_part_floats(D); };
+  constexpr int kFly = 10;  // parts of a thread in flight
+  float4 x[kFly];
+  auto fetch = [&](int i0) {
+#pragma unroll
+    for (int i = 0; i < kFly; ++i)
+      if (i0 + i * kSplit < n && quad < kQuads) x[i] = reinterpret_cast<const float4*>(part_of(i0 + i * kSplit))[quad];
+  };
+  fetch(group);
+  auto reduce = [&](float v, int what) {  // over the threads with the same row: lanes, then warps through shared memory
+    float u = __shfl_xor_sync(0xffffffffu, v, 8);
+    v = what ? v + u : fmaxf(v, u);
+    u = __shfl_xor_sync(0xffffffffu, v, 16);
+    v = what ? v + u : fmaxf(v, u);
+    if (lane < 8) red[what][tid >> 5][row] = v;
+  };
+  // the rows' common reference; a thread per (part, row)
+  float top = -INFINITY;
+  for (int i = tid >> 3; i < n; i += kJoinThreads / 8) {
+    const float* pm = part_of(i) + kDecRows * D + row;
+    const float m = pm[0];
+    if (i < kJoinParts) pml[i][0][row] = m, pml[i][1][row] = pm[kDecRows];
+    top = fmaxf(top, m);
+  }
+  reduce(top, 0);
+  __syncthreads();
+  top = -INFINITY;
+#pragma unroll
+  for (int w = 0; w < kJoinThreads / 32; ++w) top = fmaxf(top, red[0][w][row]);
+  float sum = 0.f;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int base = 0; base < n; base += kJoinParts) {
+    const int m = min(n - base, kJoinParts);
+    for (int i = tid >> 3; i < m; i += kJoinThreads / 8) {  // weights, in the place of the references
+      const float* pm = part_of(base + i) + kDecRows * D + row;
+      const float pmax = base ? pm[0] : pml[i][0][row], l = base ? pm[kDecRows] : pml[i][1][row], w = part_weight(pmax, l, top);
+      sum = fmaf(l, w, sum);
+      pml[i][0][row] = w;
+    }
+    __syncthreads();
+    for (int i0 = group; i0 < m; i0 += kFly * kSplit) {
+      if (base + i0 != group) fetch(base + i0);
+#pragma unroll
+      for (int i = 0; i < kFly; ++i) {
+        const int p = i0 + i * kSplit;
+        if (p >= m) break;
+        const float f0 = pml[p][0][2 * t], f1 = pml[p][0][2 * t + 1];
+        acc.x = fmaf(x[i].x, f0, acc.x), acc.y = fmaf(x[i].y, f1, acc.y), acc.z = fmaf(x[i].z, f0, acc.z), acc.w = fmaf(x[i].w, f1, acc.w);
+      }
+    }
+    __syncthreads();
+  }
+  reduce(sum, 1);
+  if constexpr (kSplit > 1) sums[group][tid % kEach] = acc;
+  __syncthreads();
+  if (group > 0 || quad >= kQuads) return;
+  float mm[2], ll[2] = {0.f, 0.f};
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    mm[j] = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < kJoinThreads / 32; ++w) mm[j] = fmaxf(mm[j], red[0][w][2 * t + j]), ll[j] += red[1][w][2 * t + j];
+  }
+#pragma unroll
+  for (int i = 1; i < kSplit; ++i) {
+    const float4 y = sums[i][tid];
+    acc.x += y.x, acc.y += y.y, acc.z += y.z, acc.w += y.w;
+  }
+  store_quad<T, D>(a, join.row0, join.rows, join.h, join.tile, quad, acc, mm, ll);
 }
 
 template <typename T, int D>
 int decode_init() {
-  LB_CUDA(cudaFuncSetAttribute(kv4_decode_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, dec_smem(D)));
+  LB_CUDA(cudaFuncSetAttribute(kv4_decode_kernel<T, D, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, dec_smem(D)));
+  LB_CUDA(cudaFuncSetAttribute(kv4_decode_kernel<T, D, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, dec_smem(D)));
   return LING_B200_OK;
 }
 template <typename T>
@@ -528,19 +740,35 @@ int attention_init() {
   if (const int r = decode_init_all<__nv_bfloat16>()) return r;
   return decode_init_all<__half>();
 }
+template <typename T, int D>
+int decode_launch_t(const AttnArgs& a, bool solo, int sms, cudaStream_t s) {
+  const int grid = std::min(sms, kDecMaxCtas);
+  LB_CUDA(launch_kernel(solo ? kv4_decode_kernel<T, D, true> : kv4_decode_kernel<T, D, false>, dim3(grid), dim3(kDecThreads), size_t(dec_smem(D)), s, a));
+  LB_LAUNCH("kv4_decode_kernel");
+  // of a CTA's parts there may be many to an item: four threads a quad; of a warp's there are few
+  if (solo) LB_CUDA(launch_dependent(kv4_join_kernel<T, D, 1>, dim3(grid * kDecWarps, ceil_div(2 * D, kJoinThreads)), dim3(kJoinThreads), size_t(0), s, a));
+  else LB_CUDA(launch_dependent(kv4_join_kernel<T, D, 4>, dim3(grid, D / 32), dim3(kJoinThreads), size_t(0), s, a));
+  LB_LAUNCH("kv4_join_kernel");
+  return LING_B200_OK;
+}
+// Whether warps work alone: with many (sequence, kv head, row tile) items the CTAs' meetings at every item's end cost more than
+// the partial results of single warps.
+bool decode_solo(const ling_b200_kv4& c, const ling_b200_kv4_batch& b, int q_heads) {
+  const long long tiles = ((long long)b.max_rows * (q_heads / c.kv_heads) + kDecRows - 1) / kDecRows;
+  return tiles * c.kv_heads * b.seqs >= kSoloItems;
+}
 template <typename T>
 int decode_launch(const AttnArgs& a, int sms, cudaStream_t s) {
-  auto* k = a.c.head_dim == 64 ? kv4_decode_kernel<T, 64> : a.c.head_dim == 128 ? kv4_decode_kernel<T, 128> : kv4_decode_kernel<T, 256>;
-  const int grid = std::min(sms, kDecMaxCtas);
-  LB_CUDA(launch_kernel(k, dim3(grid), dim3(kDecThreads), size_t(dec_smem(a.c.head_dim)), s, a));
-  LB_LAUNCH("kv4_decode_kernel");
-  return LING_B200_OK;
+  const bool solo = decode_solo(a.c, a.b, a.q_heads);
+  return a.c.head_dim == 64    ? decode_launch_t<T, 64>(a, solo, sms, s)
+         : a.c.head_dim == 128 ? decode_launch_t<T, 128>(a, solo, sms, s)
+                               : decode_launch_t<T, 256>(a, solo, sms, s);
 }
 
 DeviceInfo g_devices[kMaxDevices];
 std::mutex g_mutex;
 
-constexpr size_t kTicketBytes = size_t(kDecMaxCtas + 15) / 16 * 64;
+constexpr size_t kJoinBytes = kDecMaxWorkers * sizeof(Join);
 
 bool heads_ok(const ling_b200_kv4* c, int q_heads, const char* who) {
   if (q_heads >= 1 && q_heads <= 1024 && q_heads % c->kv_heads == 0) return true;
@@ -557,7 +785,7 @@ using namespace lb::d4;
 extern "C" size_t ling_b200_kv4_attention_workspace(const ling_b200_kv4* cache, const ling_b200_kv4_batch* batch, int q_heads) {
   const char* who = "kv4_attention_workspace";
   if (!kv4_cache_ok(cache, who) || !kv4_batch_ok(cache, batch, who) || !heads_ok(cache, q_heads, who)) return 0;
-  return kTicketBytes + size_t(kDecMaxCtas) * 2 * dec_part_floats(cache->head_dim) * 4;
+  return kJoinBytes + size_t(decode_solo(*cache, *batch, q_heads) ? kDecMaxWorkers : kDecMaxCtas) * 2 * dec_part_floats(cache->head_dim) * 4;
 }
 
 extern "C" int ling_b200_kv4_attention(int device, const ling_b200_kv4* cache, const ling_b200_kv4_batch* batch, int type,
@@ -575,6 +803,11 @@ extern "C" int ling_b200_kv4_attention(int device, const ling_b200_kv4* cache, c
     set_error("kv4_attention: scale must be finite, lse and err aligned");
     return LING_B200_ERR_ARG;
   }
+  const long long tiles = ((long long)batch->max_rows * (q_heads / cache->kv_heads) + kDecRows - 1) / kDecRows * cache->kv_heads;
+  if (tiles * batch->seqs > (1ll << 30) / (batch->max_context / 16 + 1)) {
+    set_error("kv4_attention: the batch's bounds (seqs x max_rows x max_context) are beyond 2^30 steps of the kernel");
+    return LING_B200_ERR_UNSUPPORTED;
+  }
   const size_t need = ling_b200_kv4_attention_workspace(cache, batch, q_heads);
   if (!workspace || workspace_bytes < need || !aligned(workspace, 16)) {
     set_error("kv4_attention: a 16-byte aligned workspace of " + std::to_string(need) + " bytes expected");
@@ -584,9 +817,9 @@ extern "C" int ling_b200_kv4_attention(int device, const ling_b200_kv4* cache, c
   DeviceGuard guard;
   int sms = 0;
   if (const int r = enter_device(guard, device, g_devices, g_mutex, attention_init, &sms)) return r;
-  AttnArgs a{*cache, *batch, *q, *out, q_heads, scale, lse, err, static_cast<unsigned*>(workspace),
-             reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + kTicketBytes), false};
-  a.q_vec = aligned(q->p, 8) && q->row % 4 == 0 && q->head % 4 == 0;
+  AttnArgs a{*cache, *batch, *q, *out, q_heads, scale, lse, err, static_cast<Join*>(workspace),
+             reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + kJoinBytes), false};
+  a.q_vec = rows_vec(*q, type);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   return type == LING_B200_BF16 ? decode_launch<__nv_bfloat16>(a, sms, s) : decode_launch<__half>(a, sms, s);
 }
