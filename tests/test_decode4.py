@@ -97,7 +97,7 @@ def c_batch(lb, **kw):
 
 
 @pytest.mark.parametrize("change", [dict(M=0), dict(M=33), dict(K=24), dict(K=0), dict(N=0), dict(ldx=31), dict(ldy=7), dict(xt=3), dict(yt=-1), dict(x=None),
-                                    dict(w=None), dict(ws=None), dict(y=None), dict(x=C.c_void_p(4097)), dict(y=C.c_void_p(4098)), dict(device=-1)])
+                                    dict(w=None), dict(ws=None), dict(y=None), dict(x=C.c_void_p(4097)), dict(y=C.c_void_p(4098)), dict(w=C.c_void_p(4100)), dict(device=-1)])
 def test_matvec_refusals(lb, change):
     a = dict(device=0, x=_p(), xt=lb.BF16, ldx=32, M=1, w=_p(2), ws=_p(3), N=8, K=32, y=_p(4), yt=lb.F32, ldy=8)
     a.update(change)
@@ -191,7 +191,7 @@ def test_matvec(gpu, lb, M, N, K, xt):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("kw", [dict(accumulate=True), dict(x_off=1), dict(x_off=8), dict(ldx=1111), dict(w_off=8), dict(w_off=3), dict(ldy=77), dict(accumulate=True, yt="f16"),
+@pytest.mark.parametrize("kw", [dict(accumulate=True), dict(x_off=1), dict(x_off=8), dict(ldx=1111), dict(w_off=8), dict(w_off=24), dict(ldy=77), dict(accumulate=True, yt="f16"),
                                 dict(xt="f32", x_off=3, ldx=1200), dict(xt="f32", accumulate=True, yt="bf16")])
 def test_matvec_strides_and_alignment(gpu, lb, kw):
     kw = dict(kw)
