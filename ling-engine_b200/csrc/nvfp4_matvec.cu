@@ -30,12 +30,11 @@ using namespace d4;
 constexpr int kWarps = 8, kThreads = kWarps * 32;
 constexpr int kUnit = 32;        // k of a unit: 16 bytes of a row
 constexpr int kChunkUnits = 8;   // units of a stage
-constexpr int kStageBytes = 32 * 128 + 32 * 20;  // 32 rows: codes; scales as the words they lie in
+constexpr int kStageBytes = 32 * 128 + 32 * 32;  // 32 rows: codes; scales, as the 16-byte pieces they lie in
 
-constexpr int kStages = 3;
-constexpr int kSumBlocks = 64;        // (tile, K part, column tile) sums of a CTA between two meetings
-constexpr int kXBytes = 82 * 1024;    // activations in shared memory
-constexpr int kSmem = kWarps * kStages * kStageBytes + kSumBlocks * 512 + kXBytes;
+constexpr int kSumBlocks = 64;   // (tile, K part, column tile) sums of a CTA between two meetings
+constexpr int kSmem = 225 * 1024;  // rings of 2 to 6 stages, sums, activations: as many stages as the rest leaves room for
+constexpr int kMaxStages = 6;
 
 struct MatvecArgs {
   const void* x;
@@ -48,7 +47,8 @@ struct MatvecArgs {
   long long ldy;
   int y_type, accumulate;
   bool x_vec;  // every row of x starts on a 16-byte boundary
-  int parts;   // warps that share a CTA's K: 1, 2, 4 or 8
+  int parts, stages;       // warps that share a CTA's K: 1, 2, 4 or 8; stages of a warp's ring
+  int tiles, more_tiles;   // tiles of a cluster; clusters that have one more
 };
 
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src, int bytes) {  // the rest of the 16 is zero
@@ -64,6 +64,15 @@ __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_grou
 template <int N>
 __device__ __forceinline__ void cp_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void cp_wait_but(int n) {  // all groups but the last n
+  switch (n) {
+    case 0: cp_wait<0>(); break;
+    case 1: cp_wait<1>(); break;
+    case 2: cp_wait<2>(); break;
+    case 3: cp_wait<3>(); break;
+    default: cp_wait<4>(); break;
+  }
 }
 __device__ __forceinline__ void mma_16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -91,74 +100,88 @@ __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_arrive_wait() { cluster_arrive(), cluster_wait(); }
 
-// Eight elements of a row from k on (zeros from K on) as floats.
-template <typename TX>
-__device__ __forceinline__ void load_x8(const TX* row, int k, int K, bool vec, float (&v)[8]) {
-  if (vec && k + 8 <= K) {
-    constexpr int kPer = 16 / sizeof(TX);
-#pragma unroll
-    for (int i = 0; i < 8 / kPer; ++i) {
-      const uint4 w = reinterpret_cast<const uint4*>(row + k)[i];
-#pragma unroll
-      for (int j = 0; j < kPer; ++j) v[i * kPer + j] = to_f32<TX>(reinterpret_cast<const TX*>(&w)[j]);
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = k + j < K ? to_f32<TX>(row[k + j]) : 0.f;
-  }
-}
+// The power of two that a row whose largest finite magnitude has these bits was multiplied by (1 / x_inv): 2^(14 - exponent).
+__device__ __forceinline__ float x_inv(uint32_t top) { return __uint_as_float(uint32_t(max(int(top >> 23) - 14, 1)) << 23); }
+__device__ __forceinline__ float x_mul(uint32_t top) { return 1.f / x_inv(top); }
 
 // kRow16: rows of codes start on 16-byte boundaries (else on 8), rows of scales on 2-byte ones (else anywhere).
 template <typename TX, int NT, bool kRow16>
 __global__ void __launch_bounds__(kThreads, 1) nvfp4_matvec_kernel(MatvecArgs a) {
   pdl_sync();  // first statement: see common.cuh
   namespace cg = cooperative_groups;
-  constexpr int S = kStages;
+  const int S = a.stages;
   constexpr bool kF32 = sizeof(TX) == 4, kScaled = !std::is_same<TX, __half>::value;
   constexpr int kCols = kF32 ? 2 : 1;  // columns of a row
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ uint32_t x_top[kWarps][8 * NT];
-  __shared__ float x_inv[8 * NT];
+  __shared__ uint32_t x_top[8 * NT];  // of a row's finite magnitudes the largest, as bits
   cg::cluster_group cluster = cg::this_cluster();
-  const int c = int(cluster.num_blocks()), rank = int(cluster.block_rank()), cid = int(blockIdx.x) / c, clusters = int(gridDim.x) / c;
+  const int c = int(cluster.num_blocks()), rank = int(cluster.block_rank()), cid = int(blockIdx.x / unsigned(c));
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-  const int parts = a.parts, part = warp % parts, groups = kWarps / parts, group = warp / parts;
+  const int parts = a.parts, lp = 31 - __clz(parts), lg = 3 - lp, part = warp & (parts - 1), group = warp >> lp;  // (powers of two)
   uint8_t* ring = smem + warp * (S * kStageBytes);
-  float4* sums = reinterpret_cast<float4*>(smem + kWarps * S * kStageBytes);  // [tile][part][column tile][lane], added into part 0
-  uint8_t* xs = smem + kWarps * S * kStageBytes + kSumBlocks * 512;
-  const uint32_t ring_u32 = static_cast<uint32_t>(__cvta_generic_to_shared(ring));
   const bool alone = c * parts == 1;  // a warp has all of K: it writes its sums itself
+  float4* sums = reinterpret_cast<float4*>(smem + kWarps * S * kStageBytes);  // [tile][part][column tile][lane], added into part 0
+  uint8_t* xs = smem + kWarps * S * kStageBytes + (alone ? 0 : kSumBlocks * 512);
+  const uint32_t ring_u32 = static_cast<uint32_t>(__cvta_generic_to_shared(ring));
 
   // ---- this cluster's weight tiles, this CTA's and this warp's units of K
-  const int tiles = (a.N + 15) / 16, units = (a.K + kUnit - 1) / kUnit;
-  const int tile0 = int((long long)tiles * cid / clusters), tile1 = int((long long)tiles * (cid + 1) / clusters);
-  const int c0 = int((long long)units * rank / c), c1 = int((long long)units * (rank + 1) / c);
-  const int u0 = c0 + (c1 - c0) * part / parts, u1 = c0 + (c1 - c0) * (part + 1) / parts;
-  const size_t row_bytes = size_t(a.K) / 2, scale_bytes = size_t(a.K) / 16;
+  const int units = (a.K + kUnit - 1) / kUnit, row_bytes = a.K / 2, scale_bytes = a.K / 16;
+  const int tile0 = a.tiles * cid + min(cid, a.more_tiles), tile1 = tile0 + a.tiles + (cid < a.more_tiles ? 1 : 0);
+  const int chunks = (units + kChunkUnits - 1) / kChunkUnits, h0 = chunks * rank / c, h1 = chunks * (rank + 1) / c;  // K is cut at whole chunks
+  const int c0 = h0 * kChunkUnits, c1 = min(units, h1 * kChunkUnits);
+  const int u0 = (h0 + ((h1 - h0) * part >> lp)) * kChunkUnits, u1 = min(units, (h0 + ((h1 - h0) * (part + 1) >> lp)) * kChunkUnits);
+  const bool scales16 = ((reinterpret_cast<uintptr_t>(a.scales) | uintptr_t(scale_bytes)) & 15) == 0;  // a chunk's scales of a row are one piece
   // Batches of tiles between meetings, of which this warp's group has the pairs [first_pair, last_pair).
-  const int batch = alone ? max(tile1 - tile0, 1) : max(kSumBlocks / (parts * NT) & ~1, 2);
-  auto first_pair = [&](int tile, int who) { return (min(batch, tile1 - tile) + 1) / 2 * who / groups; };
+  const int batch = alone ? max(tile1 - tile0, 1) : max((kSumBlocks / NT >> lp) & ~1, 2);
+  auto first_pair = [&](int tile, int who) { return ((min(batch, tile1 - tile) + 1) / 2 * who + (1 << lg) - 1) >> lg; };
+
+  // ---- the activations, asked for first: unit u, 16-byte piece q of column n lies at piece (4 u + q) ^ (u / 2 & 1 | 2 (n & 1)).  Raw at
+  // first: eight 16-bit elements where their FP16 will lie, of eight fp32 elements four where their upper parts will, four where
+  // their lower ones.
+  const int cols = a.M * kCols, x_units = max(c1 - c0, 0), x_stride = x_units * 64, x_pieces = x_units * 4, k0 = c0 * kUnit;
+  auto x_at = [&](int n, int u, int q) { return xs + n * x_stride + (((u * 4 + q) ^ ((u >> 1 & 1) | (n & 1) << 1)) * 16); };
+  if (tid < 8 * NT) x_top[tid] = 0;
+#pragma unroll 1
+  for (int m = 0, p = tid; m < a.M; p += kThreads) {
+    while (p >= x_pieces) p -= x_pieces, ++m;  // piece p of row m
+    if (m >= a.M) break;
+    const int k = k0 + p * 8;
+    const TX* src = static_cast<const TX*>(a.x) + m * a.ldx + k;
+    constexpr int kPer = 16 / sizeof(TX);
+#pragma unroll
+    for (int j = 0; j < kCols; ++j) {
+      uint8_t* to = x_at(m * kCols + j, p >> 2, p & 3);
+      if (a.x_vec) {  // (K is a multiple of 16: a piece is there whole or not at all)
+        cp16(static_cast<uint32_t>(__cvta_generic_to_shared(to)), k < a.K ? src + j * kPer : static_cast<const TX*>(a.x), k < a.K ? 16 : 0);
+      } else {
+#pragma unroll 1
+        for (int e = 0; e < kPer; ++e) reinterpret_cast<TX*>(to)[e] = k < a.K ? src[j * kPer + e] : TX(0.f);
+      }
+    }
+  }
+  cp_commit();
 
   // ---- the loading side: batch by batch, pair of tiles by pair, chunk of 8 units by chunk
   int in_tile = tile0, in_pair = first_pair(tile0, group), in_last = first_pair(tile0, group + 1), in_unit = u0, put = 0;
   const int r = lane >> 3, cu = lane & 7;  // copied: row r (of four) and unit cu of a stage's 8
   auto issue = [&]() {
+    if (u0 >= u1) in_tile = tile1;
     while (in_pair == in_last && in_tile < tile1) {
       in_tile += batch;
       if (in_tile < tile1) in_pair = first_pair(in_tile, group), in_last = first_pair(in_tile, group + 1);
     }
-    if (in_tile < tile1 && u0 < u1) {
+    if (in_tile < tile1) {
       const int n = min(kChunkUnits, u1 - in_unit);
       const int row0 = (in_tile + in_pair * 2) * 16, rows = min(a.N, tile1 * 16) - row0;  // rows that are there
       const uint32_t st = ring_u32 + put * kStageBytes;
       // codes: four rows an instruction; unit u of row r lies at u ^ 4 (r & 1)
-      const uint8_t* src = a.values + size_t(row0 + r) * row_bytes + size_t(in_unit + cu) * 16;
+      const uint8_t* src = a.values + size_t(row0 + r) * row_bytes + (in_unit + cu) * 16;
       const uint32_t dst = st + r * 128 + ((cu ^ (r & 1) * 4) * 16);
       if (kRow16 && rows >= 32 && n == kChunkUnits) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) cp16(dst + i * 512, src + size_t(i * 4) * row_bytes, 16);
       } else {
-        const int left = cu < n ? int(min((long long)row_bytes - (long long)(in_unit + cu) * 16, 16ll)) : 0;
+        const int left = cu < n ? min(row_bytes - (in_unit + cu) * 16, 16) : 0;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           const bool there = i * 4 + r < rows && left > 0;
@@ -171,92 +194,89 @@ __global__ void __launch_bounds__(kThreads, 1) nvfp4_matvec_kernel(MatvecArgs a)
           }
         }
       }
-      // scales: a row a lane, the words that hold at least one of its bytes
-      const int bytes = lane < rows ? int(min((long long)scale_bytes - (long long)in_unit * 2, (long long)n * 2)) : 0;
-      const uintptr_t at = reinterpret_cast<uintptr_t>(a.scales) + size_t(row0 + (lane < rows ? lane : 0)) * scale_bytes + size_t(in_unit) * 2;
-      const uint8_t* w = reinterpret_cast<const uint8_t*>(at & ~uintptr_t(3));
-      const int end = bytes > 0 ? int(at & 3) + bytes : 0;
-#pragma unroll
-      for (int i = 0; i < 5; ++i) cp4(st + 32 * 128 + lane * 20 + i * 4, i * 4 < end ? w + i * 4 : w, i * 4 < end ? 4 : 0);
+      // scales: a row a lane, the one or two 16-byte pieces that hold at least one of its bytes
+      const int bytes = lane < rows ? min(scale_bytes - in_unit * 2, n * 2) : 0;
+      const uintptr_t at = reinterpret_cast<uintptr_t>(a.scales) + size_t(row0 + (lane < rows ? lane : 0)) * scale_bytes + in_unit * 2;
+      const uint8_t* w = reinterpret_cast<const uint8_t*>(at & ~uintptr_t(15));
+      cp16(st + 32 * 128 + lane * 32, w, bytes > 0 ? 16 : 0);
+      if (!scales16) {
+        const bool two = bytes > 0 && int(at & 15) + bytes > 16;
+        cp16(st + 32 * 128 + lane * 32 + 16, two ? w + 16 : w, two ? 16 : 0);
+      }
       put = put + 1 == S ? 0 : put + 1;
       in_unit += n;
       if (in_unit == u1) in_unit = u0, ++in_pair;
     }
     cp_commit();
   };
-#pragma unroll
+#pragma unroll 1
   for (int i = 0; i < S - 1; ++i) issue();
 
-  // ---- the activations as FP16 columns: unit u, 16-byte piece q of column n lies at piece (4 u + q) ^ (u / 2 & 1 | 2 (n & 1))
-  const int cu_n = c1 - c0, x_stride = cu_n * 64;
-  auto x_at = [&](int n, int u, int q) { return xs + n * x_stride + (((u * 4 + q) ^ ((u >> 1 & 1) | (n & 1) << 1)) * 16); };
-  {
-    constexpr int kRows = NT == 1 ? (kF32 ? 2 : 4) : 4, kFly = NT == 1 ? 3 : NT == 2 ? 2 : 1;  // rows in flight, 8-element pieces of a thread
-    const int pieces = cu_n * 4, k0 = c0 * kUnit;
-    for (int m0 = 0; m0 < a.M; m0 += kRows) {
-      float v[kRows][kFly][8];
+  // ---- the activations to FP16, in place: a warp takes a row, or a part of it where there are few
+  cp_wait_but(S - 1);
+  __syncthreads();
+  if constexpr (kScaled) {
+    const int segments = a.M >= kWarps ? 1 : a.M == 1 ? kWarps : kWarps / a.M, per = (x_pieces + segments - 1) / segments;
+#pragma unroll 1
+    for (int i = warp; i < a.M * segments; i += kWarps) {
+      const int m = i / segments, p0 = (i - m * segments) * per, p1 = min(x_pieces, p0 + per);
+      uint32_t top = 0;
+#pragma unroll 1
+      for (int p = p0 + lane; p < p1; p += 32)
 #pragma unroll
-      for (int i = 0; i < kRows; ++i)
+        for (int j = 0; j < kCols; ++j) {
+          const uint4 w = *reinterpret_cast<const uint4*>(x_at(m * kCols + j, p >> 2, p & 3));
+          const uint32_t e[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-        for (int j = 0; j < kFly; ++j)
-          if (m0 + i < a.M && tid + j * kThreads < pieces) load_x8(static_cast<const TX*>(a.x) + (m0 + i) * a.ldx, k0 + (tid + j * kThreads) * 8, a.K, a.x_vec, v[i][j]);
-      if constexpr (kScaled) {
-#pragma unroll
-        for (int i = 0; i < kRows; ++i) {
-          uint32_t top = 0;  // bits of the largest finite magnitude
-#pragma unroll
-          for (int j = 0; j < kFly; ++j)
-            if (m0 + i < a.M && tid + j * kThreads < pieces) {
-#pragma unroll
-              for (int e = 0; e < 8; ++e) {
-                const uint32_t b = __float_as_uint(v[i][j][e]) & 0x7fffffffu;
-                top = b < 0x7f800000u ? max(top, b) : top;
-              }
-            }
-          top = __reduce_max_sync(0xffffffffu, top);
-          if (lane == 0 && m0 + i < a.M) x_top[warp][m0 + i] = top;
-        }
-        __syncthreads();
-      }
-#pragma unroll
-      for (int i = 0; i < kRows; ++i) {
-        if (m0 + i >= a.M) break;
-        float mul = 1.f, inv = 1.f;
-        if constexpr (kScaled) {
-          uint32_t top = 0;
-#pragma unroll
-          for (int w = 0; w < kWarps; ++w) top = max(top, x_top[w][m0 + i]);
-          inv = __uint_as_float(uint32_t(max(int(top >> 23) - 14, 1)) << 23);  // 2^(exponent - 14)
-          mul = 1.f / inv;
-        }
-#pragma unroll
-        for (int j = 0; j < kFly; ++j) {
-          const int p = tid + j * kThreads;
-          if (p >= pieces) continue;
-          uint32_t hi[4], lo[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float e0 = v[i][j][2 * e] * mul, e1 = v[i][j][2 * e + 1] * mul;
-            hi[e] = h2(e0, e1);
+          for (int q = 0; q < 4; ++q) {
             if constexpr (kF32) {
-              const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hi[e]));
-              lo[e] = h2(fabsf(e0) < INFINITY ? e0 - f.x : 0.f, fabsf(e1) < INFINITY ? e1 - f.y : 0.f);
+              const uint32_t b = e[q] & 0x7fffffffu;
+              top = b < 0x7f800000u ? max(top, b) : top;
+            } else {
+              const uint32_t b0 = e[q] << 16 & 0x7fffffffu, b1 = e[q] & 0x7fff0000u;
+              top = b0 < 0x7f800000u ? max(top, b0) : top, top = b1 < 0x7f800000u ? max(top, b1) : top;
             }
           }
-          *reinterpret_cast<uint4*>(x_at((m0 + i) * kCols, p >> 2, p & 3)) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-          if constexpr (kF32) *reinterpret_cast<uint4*>(x_at((m0 + i) * kCols + 1, p >> 2, p & 3)) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
         }
-        if (tid < kCols) x_inv[(m0 + i) * kCols + tid] = inv;
+      top = __reduce_max_sync(0xffffffffu, top);
+      if (lane == 0) atomicMax(&x_top[m], top);
+    }
+    __syncthreads();
+#pragma unroll 1
+    for (int m = 0, p = tid; m < a.M; p += kThreads) {
+      while (p >= x_pieces) p -= x_pieces, ++m;
+      if (m >= a.M) break;
+      const float mul = x_mul(x_top[m]);
+      uint4* hi = reinterpret_cast<uint4*>(x_at(m * kCols, p >> 2, p & 3));
+      const uint4 w = *hi;
+      if constexpr (kF32) {
+        uint4* lo = reinterpret_cast<uint4*>(x_at(m * kCols + 1, p >> 2, p & 3));
+        const uint4 v = *lo;
+        const uint32_t e[8] = {w.x, w.y, w.z, w.w, v.x, v.y, v.z, v.w};
+        uint32_t h[4], l[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const float e0 = __uint_as_float(e[2 * q]) * mul, e1 = __uint_as_float(e[2 * q + 1]) * mul;
+          h[q] = h2(e0, e1);
+          const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h[q]));
+          l[q] = h2(fabsf(e0) < INFINITY ? e0 - f.x : 0.f, fabsf(e1) < INFINITY ? e1 - f.y : 0.f);
+        }
+        *hi = make_uint4(h[0], h[1], h[2], h[3]), *lo = make_uint4(l[0], l[1], l[2], l[3]);
+      } else {
+        const uint32_t e[4] = {w.x, w.y, w.z, w.w};
+        uint32_t h[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) h[q] = h2(__uint_as_float(e[q] << 16) * mul, __uint_as_float(e[q] & 0xffff0000u) * mul);
+        *hi = make_uint4(h[0], h[1], h[2], h[3]);
       }
     }
-    for (int i = tid; i < (8 * NT - a.M * kCols) * cu_n * 4; i += kThreads)  // columns that are not there
-      *reinterpret_cast<uint4*>(xs + a.M * kCols * x_stride + i * 16) = make_uint4(0, 0, 0, 0);
-    for (int i = a.M * kCols + tid; i < 8 * NT; i += kThreads) x_inv[i] = 1.f;
+    __syncthreads();
   }
-  __syncthreads();
   float inv[NT][2];
 #pragma unroll
-  for (int n = 0; n < NT; ++n) inv[n][0] = x_inv[n * 8 + 2 * t], inv[n][1] = x_inv[n * 8 + 2 * t + 1];
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int j = 0; j < 2; ++j) inv[n][j] = kScaled ? x_inv(x_top[(n * 8 + 2 * t + j) / kCols]) : 1.f;
 
   // Writes quad v of (tile, column tile): rows g and g + 8, columns 2t and 2t + 1.
   auto write_quad = [&](int tile, int nn, const float4& s) {
@@ -273,6 +293,12 @@ __global__ void __launch_bounds__(kThreads, 1) nvfp4_matvec_kernel(MatvecArgs a)
       }
   };
 
+  // this thread's columns (one that is not there is never written: any stands in); a chunk starts at a multiple of 8 units, so where
+  // a piece lies in its unit depends on the thread alone
+  const uint8_t* x_col[NT];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) x_col[n] = xs + min(n * 8 + g, cols - 1) * x_stride;
+  const int x_swizzle = t >> 1 | (g & 1) << 1;
   int stage = 0;
   bool read_pending = false;  // the other CTAs may still be reading this one's sums
   for (int tile = tile0; tile < tile1; tile += batch) {
@@ -281,7 +307,7 @@ __global__ void __launch_bounds__(kThreads, 1) nvfp4_matvec_kernel(MatvecArgs a)
       float acc[2][NT][4] = {};
       for (int unit = u0; unit < u1; unit += kChunkUnits) {
         const int n_units = min(kChunkUnits, u1 - unit);
-        cp_wait<S - 2>();
+        cp_wait_but(S - 2);
         __syncwarp();  // the stage has landed, for all lanes; all lanes are done with the one before, whose place is next
         issue();
         const uint8_t* st = ring + stage * kStageBytes;
@@ -292,18 +318,18 @@ __global__ void __launch_bounds__(kThreads, 1) nvfp4_matvec_kernel(MatvecArgs a)
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
             const int row = i * 16 + half * 8 + g;
-            const uint32_t byte = uint32_t(reinterpret_cast<uintptr_t>(a.scales)) + uint32_t((tile + pair * 2) * 16 + row) * uint32_t(scale_bytes) + uint32_t(unit) * 2u;
-            row_s[i][half] = st + 32 * 128 + row * 20 + (byte & 3u) + t * 2;
+            row_s[i][half] = st + 32 * 128 + row * 32 + t * 2;
+            if (!scales16) row_s[i][half] += (uint32_t(reinterpret_cast<uintptr_t>(a.scales)) + uint32_t((tile + pair * 2) * 16 + row) * uint32_t(scale_bytes) + uint32_t(unit) * 2u) & 15u;
           }
-        const uint8_t* row_w = st + g * 128;
+        const uint8_t* row_w = st + g * 128 + t * 16;
+        const int x_off = (unit - c0) * 64;
         auto piece = [&](int p, bool here) {  // four units, this thread's being unit + 4 p + t; !here: it is not in the chunk
-          const int u = unit - c0 + (here ? p * 4 + t : 0);
           uint32_t w[2][2][4], sc[2][2][2];  // codes; scales of the two groups
 #pragma unroll
           for (int i = 0; i < 2; ++i)
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
-              const uint4 v = *reinterpret_cast<const uint4*>(row_w + (i * 16 + half * 8) * 128 + (((p * 4 + t) ^ (g & 1) * 4) * 16));
+              const uint4 v = *reinterpret_cast<const uint4*>(row_w + (i * 16 + half * 8) * 128 + ((p ^ (g & 1)) * 64));
               w[i][half][0] = v.x, w[i][half][1] = v.y, w[i][half][2] = v.z, w[i][half][3] = v.w;
               const uint8_t* at_s = row_s[i][half] + p * 8;
               uint32_t two;
@@ -317,7 +343,7 @@ __global__ void __launch_bounds__(kThreads, 1) nvfp4_matvec_kernel(MatvecArgs a)
             uint4 xf[NT];
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-              xf[n] = *reinterpret_cast<const uint4*>(x_at(n * 8 + g, u, j));
+              xf[n] = *reinterpret_cast<const uint4*>(x_col[n] + (here ? x_off + p * 256 + t * 64 : 0) + ((j ^ x_swizzle) * 16));
               if (!here) xf[n] = make_uint4(0, 0, 0, 0);
             }
 #pragma unroll
@@ -363,10 +389,13 @@ __global__ void __launch_bounds__(kThreads, 1) nvfp4_matvec_kernel(MatvecArgs a)
     if (c > 1 && read_pending) cluster_wait(), read_pending = false;
     __syncthreads();
     if (parts > 1) {
+#pragma unroll 1
       for (int i = tid; i < batch_tiles * NT * 32; i += kThreads) {
         float4* at = sums + size_t(i / (NT * 32)) * (parts * NT * 32) + i % (NT * 32);
         float4 s = *at;
-        for (int p = 1; p < parts; ++p) {
+#pragma unroll
+        for (int p = 1; p < kWarps; ++p) {
+          if (p >= parts) break;
           const float4 v = at[p * NT * 32];
           s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
         }
@@ -376,6 +405,7 @@ __global__ void __launch_bounds__(kThreads, 1) nvfp4_matvec_kernel(MatvecArgs a)
     }
     if (c > 1) {
       cluster_arrive_wait();
+#pragma unroll 1
       for (int block = rank + warp * c; block < batch_tiles * NT; block += kWarps * c) {
         float4* at = sums + size_t(block / NT) * (parts * NT * 32) + block % NT * 32 + lane;
         float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -433,27 +463,31 @@ int init_all(int device) {
   return init_type<__half>(g_clusters[device]);
 }
 
-// CTAs and warps that share K: the split with the least estimated time.  A warp's stage streams at about 5.5 bytes a nanosecond (its
-// share of HBM) but takes 250 ns at least; a meeting costs about 0.7 us, of a cluster's CTAs 2 us.  false: the activations of
-// `nt` column tiles fit no split.
+// CTAs and warps that share K: the split with the least estimated time.  A warp's stage takes its share of the SM's part of HBM (4736
+// bytes at 5.5 a nanosecond), or the loaded latency of about 2 us over the stages in flight, or its instructions (about 700 ns and
+// 150 a column tile beyond the first); a meeting costs about 0.7 us, of a cluster's CTAs 2 us.  false: `cols` columns of activations (in
+// `nt` tiles of 8) fit no split.
 struct Split {
-  int c = 0, parts = 0, clusters = 0;
+  int c = 0, parts = 0, clusters = 0, stages = 0;
 };
-bool choose_split(const int* at_once, int N, int K, int nt, Split* out) {
-  const int tiles = ceil_div(N, 16), units = ceil_div(K, kUnit);
+bool choose_split(const int* at_once, int N, int K, int nt, int cols, Split* out) {
+  const int tiles = ceil_div(N, 16), chunks = ceil_div(K, kUnit * kChunkUnits);
   double best = 0;
   for (int i = 0; i < 4; ++i) {
-    const int c = 1 << i, clusters = std::min(at_once[i], tiles), cta_units = ceil_div(units, c);
-    if (cta_units * 64 * 8 * nt > kXBytes || (i > 0 && units < c)) continue;
+    const int c = 1 << i, clusters = std::min(at_once[i], tiles), cta_chunks = ceil_div(chunks, c);
+    if (i > 0 && chunks < c) continue;
     for (int parts = 1; parts <= kWarps; parts *= 2) {
-      const int groups = kWarps / parts, t = ceil_div(tiles, clusters), u = ceil_div(cta_units, parts);
+      const int room = kSmem - cta_chunks * kChunkUnits * 64 * cols - (c * parts == 1 ? 0 : kSumBlocks * 512), stages = std::min(kMaxStages, room / (kWarps * kStageBytes));
+      if (room < 0 || stages < 2) continue;
+      const int groups = kWarps / parts, t = ceil_div(tiles, clusters), h = ceil_div(cta_chunks, parts);
       const int batch = c * parts == 1 ? t : std::max(kSumBlocks / (parts * nt) & ~1, 2);
+      const double full = std::max({861.0, 2000.0 / (stages - 1), 700.0 + 150.0 * (nt - 1)});
       double cost = 0;
       for (int left = t; left > 0; left -= batch) {
         const int pairs = ceil_div(ceil_div(std::min(left, batch), 2), groups);
-        cost += pairs * (u / kChunkUnits * 840.0 + (u % kChunkUnits ? std::max(250.0, u % kChunkUnits * 105.0) : 0.0)) + (c > 1 ? 2000.0 : parts > 1 ? 700.0 : 0.0);
+        cost += pairs * h * full + (c > 1 ? 2000.0 : parts > 1 ? 700.0 : 0.0);
       }
-      if (!out->c || cost < best) best = cost, *out = Split{c, parts, clusters};
+      if (!out->c || cost < best) best = cost, *out = Split{c, parts, clusters, stages};
     }
   }
   return out->c != 0;
@@ -462,7 +496,8 @@ bool choose_split(const int* at_once, int N, int K, int nt, Split* out) {
 template <typename TX, int NT>
 int matvec_launch(MatvecArgs a, const Split& split, cudaStream_t s) {
   const bool row16 = a.K % 32 == 0 && aligned(a.values, 16) && aligned(a.scales, 2);
-  a.parts = split.parts;
+  a.parts = split.parts, a.stages = split.stages;
+  a.tiles = ceil_div(a.N, 16) / split.clusters, a.more_tiles = ceil_div(a.N, 16) % split.clusters;
   LB_CUDA(launch_kernel_cluster(row16 ? nvfp4_matvec_kernel<TX, NT, true> : nvfp4_matvec_kernel<TX, NT, false>, dim3(split.clusters * split.c),
                                 dim3(kThreads), size_t(kSmem), split.c, s, a));
   LB_LAUNCH("nvfp4_matvec_kernel");
@@ -476,9 +511,9 @@ int matvec_rows(MatvecArgs a, int device, cudaStream_t s) {
   for (int m = 0, rows; m < a.M; m += rows) {
     MatvecArgs b = a;
     Split split;
-    int nt = 4;
-    while (nt > 1 && (a.M - m) * kCols <= 4 * nt) nt /= 2;
-    while (!choose_split(g_clusters[device], a.N, a.K, nt, &split)) {
+    int nt = 4, left = (a.M - m) * kCols;
+    while (nt > 1 && left <= 4 * nt) nt /= 2;
+    while (!choose_split(g_clusters[device], a.N, a.K, nt, std::min(left, 8 * nt), &split)) {
       if (nt == 1) {
         set_error("nvfp4_matvec: K = " + std::to_string(a.K) + " is beyond the activations' shared memory");
         return LING_B200_ERR_UNSUPPORTED;
@@ -513,7 +548,7 @@ extern "C" int ling_b200_nvfp4_matvec(int device, const void* x, int x_type, lon
   d4::DeviceGuard guard;
   int sms = 0;
   if (const int r = d4::enter_device(guard, device, g_devices, g_mutex, [device] { return init_all(device); }, &sms)) return r;
-  MatvecArgs a{x, ldx, M, values, scales, alpha, N, K, y, ldy, y_type, accumulate, false, 1};
+  MatvecArgs a{x, ldx, M, values, scales, alpha, N, K, y, ldy, y_type, accumulate, false, 1, 2, 0, 0};
   a.x_vec = d4::aligned(x, 16) && ldx * d4::type_size(x_type) % 16 == 0;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   return x_type == LING_B200_F32 ? matvec_rows<float>(a, device, s)
