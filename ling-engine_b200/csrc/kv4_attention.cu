@@ -6,6 +6,7 @@
 #include <algorithm>
 
 #include "decode4.cuh"
+#include "tc.cuh"
 
 namespace lb {
 namespace {
@@ -25,7 +26,7 @@ struct AttnArgs {
   int* err;
   Join* joins;
   float* parts;
-  bool q_vec;  // rows of q start on 16-byte boundaries
+  bool q_vec, out_vec;  // rows of q, of out start on 16-byte boundaries
 };
 
 // ---------------------------------------------------------------------------------------------- few query rows
@@ -724,9 +725,497 @@ __global__ void __launch_bounds__(kJoinThreads) kv4_join_kernel(AttnArgs a) {
   store_quad<T, D>(a, join.row0, join.rows, join.h, join.tile, quad, acc, mm, ll);
 }
 
+// ---------------------------------------------------------------------------------------------- many query rows
+// The tile kernel: 128 query rows of one (sequence, kv head) against its keys, 128 at a time, on tcgen05.mma kind::f16 with the
+// accumulators in TMEM.  Roles:
+//   warps 4..11  turn a tile's codes into FP16 operands in 128B-swizzled shared memory, keys as rows: K as the score product's
+//                K-major B operand, V, in the same layout, as the value product's MN-major one (no transposition).  Their
+//                loads run one tile ahead in registers, the page ids two.
+//   warp 12      one thread issues the MMAs: S(t+1) = Q K(t+1)^T before O += P(t) V(t), S double in TMEM, so that the tensor
+//                core works while the softmax of the tile in between runs.
+//   warps 0..3   a thread a row (its TMEM lane): maximum, probabilities to FP16 in shared memory, sum; O is scaled in TMEM only when
+//                a score exceeds the row's reference by 2^kLazy.
+// What bounds it is shared memory: operands are read once by the MMAs and written once by the converting warps (D = 256: 224 KB
+// and 160 KB a tile, 3072 cycles at 128 bytes, against 2048 cycles of MMA).
+// Every wait is bounded; one that runs out is recorded and the CTA leaves with its TMEM freed.
+constexpr int kTileRows = 128, kTileKeys = 128, kTileThreads = 13 * 32, kTileWorkers = 256, kTileMarks = 8;
+template <int D>
+struct TileSmem {
+  static constexpr int kOperand = 256 * D;  // 128 rows of D halves: [D / 64][128][128 B]
+  static constexpr int kP = 2 * 128 * 128;  // [2][128 rows][128 B]
+  static constexpr int kBytes = 3 * kOperand + kP + 1024;
+};
+__host__ __device__ constexpr size_t tile_part_floats(int D) { return size_t(kTileRows) * D + 2 * kTileRows; }
+
+// Shared-memory descriptor of an MN-major operand under the 128B swizzle: rows are k, 128 bytes (64 elements of mn) each; eight rows are
+// 1024 bytes apart (stride offset), blocks of 64 mn `lead` bytes (leading offset).
+__device__ __forceinline__ uint64_t desc_mn_sw128(uint32_t addr, uint32_t lead) {
+  return uint64_t((addr & 0x3FFFFu) >> 4) | uint64_t(lead >> 4) << 16 | uint64_t(1024 >> 4) << 32 | uint64_t(1) << 46 | uint64_t(2) << 61;
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kTileThreads, 1) kv4_tile_kernel(AttnArgs a, int splits) {
+  pdl_sync();  // first statement: see common.cuh
+  using namespace tc;
+  constexpr int kOperand = TileSmem<D>::kOperand, kBlocks = D / 64, kUnits = D / 64;  // 32-dim units of a key a worker converts per tile
+  constexpr uint32_t kOcol = 2 * kTileKeys;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* qs = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  uint8_t* ks = qs + kOperand;
+  uint8_t* vs = ks + kOperand;
+  uint8_t* ps = vs + kOperand;
+  __shared__ uint64_t k_full, v_full, qk_done[2], p_full, pv_done;  // (two score barriers: the next tile's may be done before this one's is waited for)
+  __shared__ uint32_t tmem_slot, bad_keys[kTileMarks][4], nan_keys[kTileMarks][4];  // by tile: keys on bad pages; (masked tiles) keys whose V is NaN
+  __shared__ float q_inv[kTileRows];
+  __shared__ int where[2];
+  __shared__ volatile int failed;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int G = a.q_heads / a.c.kv_heads, H = a.c.kv_heads, h = blockIdx.y, lp = 31 - __clz(a.c.page_tokens);
+
+  // ---- which 128 query rows: the long contexts' (later tiles) first
+  const int index = int(gridDim.x) - 1 - int(blockIdx.x);
+  if (warp == 0) {
+    int before = 0, found = -1, found_tile = 0;
+    for (int s0 = 0; s0 < a.b.seqs && found < 0; s0 += 32) {
+      const int s = s0 + lane;
+      int n = 0;
+      if (s < a.b.seqs) {
+        const Kv4Seq q = kv4_seq(a.c, a.b, s);
+        if (!q.ok && blockIdx.x == 0 && blockIdx.y == 0 && blockIdx.z == 0) dev_fail(a.err, kDevBadBatch);
+        n = q.ok ? (q.n * G + kTileRows - 1) / kTileRows : 0;
+      }
+      int end = n;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, end, o);
+        if (lane >= o) end += v;
+      }
+      end += before;
+      const unsigned mine = __ballot_sync(0xffffffffu, index >= end - n && index < end);
+      if (mine) {
+        found = s0 + __ffs(mine) - 1;
+        found_tile = index - __shfl_sync(0xffffffffu, end - n, __ffs(mine) - 1);
+      }
+      before = __shfl_sync(0xffffffffu, end, 31);
+    }
+    if (lane == 0) where[0] = found, where[1] = found_tile;
+  }
+  if (tid == 0) {
+    mbar_init(&k_full, kTileWorkers / 32);
+    mbar_init(&v_full, kTileWorkers / 32);
+    mbar_init(&qk_done[0], 1);
+    mbar_init(&qk_done[1], 1);
+    mbar_init(&p_full, 4);
+    mbar_init(&pv_done, 1);
+    failed = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (tid < kTileMarks * 4) (&bad_keys[0][0])[tid] = 0, (&nan_keys[0][0])[tid] = 0;
+  __syncthreads();
+  if (where[0] < 0) return;
+  const Kv4Seq sq = kv4_seq(a.c, a.b, where[0]);
+  const int f0 = where[1] * kTileRows, R = sq.n * G;  // this block's query rows f0 .. f0 + 127 of R: row f is (row f / G, head f % G)
+  const int last_i = min(f0 + kTileRows, R) - 1;
+  const int keys = a.b.anc ? sq.pos + sq.n : sq.pos + last_i / G + 1;             // no row sees further
+  const int all_see = a.b.anc ? sq.pos : sq.pos + f0 / G + 1;                     // every row sees at least these
+  const int tiles = (keys + kTileKeys - 1) / kTileKeys;
+  const int t0 = int((long long)tiles * blockIdx.z / splits), nt = int((long long)tiles * (blockIdx.z + 1) / splits) - t0;
+  float* part = a.parts + ((size_t(index) * H + h) * splits + blockIdx.z) * tile_part_floats(D);
+  if (nt == 0) {  // (more splits than tiles)
+    if (tid < kTileRows) part[kTileRows * D + tid] = -INFINITY, part[kTileRows * D + kTileRows + tid] = 0.f;
+    return;
+  }
+  if (warp == 12) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(512) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    tc_fence_before();
+  }
+  // ---- Q to FP16, each row times 2^(8 - exponent of its largest value) and the scale's sign (a row with a value that is not finite
+  // becomes NaN): D / 8 lanes a row
+  {
+    constexpr int kLanes = D / 8, kRowsAtOnce = 32 / kLanes, kFly = 4;
+    const int sub = lane / kLanes, piece = lane % kLanes;
+    for (int r0 = warp * kRowsAtOnce * kFly; r0 < kTileRows; r0 += 13 * kRowsAtOnce * kFly) {
+      uint4 w[kFly];
+#pragma unroll
+      for (int i = 0; i < kFly; ++i) {
+        const int r = r0 + i * kRowsAtOnce + sub, f = f0 + r;
+        w[i] = make_uint4(0, 0, 0, 0);
+        if (r < kTileRows && f < R) {
+          const T* src = static_cast<const T*>(a.q.p) + (sq.row0 + f / G) * a.q.row + (h * G + f % G) * a.q.head + piece * 8;
+          if (a.q_vec) {
+            w[i] = *reinterpret_cast<const uint4*>(src);
+          } else {
+            const uint16_t* e = reinterpret_cast<const uint16_t*>(src);
+            w[i] = make_uint4(e[0] | uint32_t(e[1]) << 16, e[2] | uint32_t(e[3]) << 16, e[4] | uint32_t(e[5]) << 16, e[6] | uint32_t(e[7]) << 16);
+          }
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < kFly; ++i) {
+        const int r = r0 + i * kRowsAtOnce + sub;
+        uint32_t top2 = __vmaxu2(__vmaxu2(w[i].x & 0x7fff7fffu, w[i].y & 0x7fff7fffu), __vmaxu2(w[i].z & 0x7fff7fffu, w[i].w & 0x7fff7fffu));
+#pragma unroll
+        for (int o = 1; o < kLanes; o <<= 1) top2 = __vmaxu2(top2, __shfl_xor_sync(0xffffffffu, top2, o));
+        const uint16_t bits = uint16_t(max(top2 & 0xffffu, top2 >> 16));
+        const float top = to_f32<T>(*reinterpret_cast<const T*>(&bits));
+        const int field = min(max(262 - int(__float_as_uint(top) >> 23 & 255u), 2), 252);
+        const float mul = (a.scale < 0.f ? -1.f : 1.f) * (top == 0.f ? 1.f : top < INFINITY ? __uint_as_float(uint32_t(field) << 23) : NAN);
+        const uint32_t e[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+        uint32_t o[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const T* two = reinterpret_cast<const T*>(&e[j]);
+          o[j] = h2(to_f32<T>(two[0]) * mul, to_f32<T>(two[1]) * mul);
+        }
+        if (r < kTileRows) {
+          *reinterpret_cast<uint4*>(qs + (piece >> 3) * (kTileRows * 128) + sw128_offset(r, piece & 7)) = make_uint4(o[0], o[1], o[2], o[3]);
+          if (piece == 0) q_inv[r] = top > 0.f && top < INFINITY ? __uint_as_float(uint32_t(254 - field) << 23) : 1.f;
+        }
+      }
+    }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_slot;
+  auto wait = [&](uint64_t* bar, int n, int code) {  // the n-th completion (n < 0: none to wait for); false: give up
+    if (n < 0 || mbar_wait(bar, uint32_t(n) & 1u, &failed)) return true;
+    dev_fail(a.err, code);
+    failed = 1;
+    return false;
+  };
+
+  if (warp == 12) {
+    // ---------------------------------------------------------------- the MMAs
+    if (lane == 0) {
+      constexpr uint32_t kIdescS = umma_idesc_f16(kTileKeys), kIdescO = umma_idesc_f16(D) | 1u << 16;  // (bit 16: B is MN-major)
+      auto scores = [&](int t) {
+        if (!wait(&k_full, t, kDevWaitFull)) return false;
+        tc_fence_after();
+#pragma unroll
+        for (int b = 0; b < kBlocks; ++b)
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            umma_f16(tmem + uint32_t(t & 1) * kTileKeys, umma_desc_sw128(smem_u32(qs + b * (kTileRows * 128))) + uint64_t(k * 2),
+                     umma_desc_sw128(smem_u32(ks + b * (kTileKeys * 128))) + uint64_t(k * 2), kIdescS, (b | k) ? 1u : 0u);
+        umma_commit(&qk_done[t & 1]);
+        return true;
+      };
+      bool ok = scores(0);
+      for (int t = 0; t < nt && ok; ++t) {
+        if (t + 1 < nt) ok = scores(t + 1);
+        ok = ok && wait(&p_full, t, kDevWaitFull) && wait(&v_full, t, kDevWaitFull);
+        if (!ok) break;
+        tc_fence_after();
+#pragma unroll
+        for (int k = 0; k < kTileKeys / 16; ++k)
+          umma_f16(tmem + kOcol, umma_desc_sw128(smem_u32(ps + (k >> 2) * (kTileRows * 128))) + uint64_t((k & 3) * 2),
+                   desc_mn_sw128(smem_u32(vs + k * 16 * 128), kTileKeys * 128), kIdescO, (t | k) ? 1u : 0u);
+        umma_commit(&pv_done);
+      }
+    }
+    __syncwarp();
+  } else if (warp >= 4) {
+    // ---------------------------------------------------------------- the operands
+    const int w = tid - 128, unit = w % (D / 32), key0 = w / (D / 32);  // units of 32 dims: keys key0, key0 + 256 / (D / 32), ..
+    constexpr int kKeyStep = kTileWorkers / (D / 32);
+    const int* table = a.c.tables + size_t(sq.slot) * a.c.max_pages;
+    struct Codes {
+      uint4 c[kUnits];
+      uint16_t s[kUnits];
+    };
+    int page[kUnits];  // of the tile after the one whose codes are asked for
+    auto look_up = [&](int t) {
+#pragma unroll
+      for (int u = 0; u < kUnits; ++u) {
+        const int pos = (t0 + t) * kTileKeys + key0 + u * kKeyStep;
+        page[u] = t < nt && pos < keys ? table[pos >> lp] : -1;
+      }
+    };
+    auto ask = [&](const uint8_t* codes, const uint8_t* scales, int t, const int (&pg)[kUnits], Codes& x) {
+#pragma unroll
+      for (int u = 0; u < kUnits; ++u) {
+        const int pos = (t0 + t) * kTileKeys + key0 + u * kKeyStep;
+        x.c[u] = make_uint4(0, 0, 0, 0), x.s[u] = 0;
+        if (pg[u] >= 1 && pg[u] <= a.c.pages) {
+          const size_t vec = ((size_t(pg[u]) * H + h) << lp) + (pos & ((1 << lp) - 1));
+          x.c[u] = *reinterpret_cast<const uint4*>(codes + vec * (D / 2) + unit * 16);
+          x.s[u] = *reinterpret_cast<const uint16_t*>(scales + vec * (D / 16) + unit * 2);
+        }
+      }
+    };
+    auto convert = [&](uint8_t* to, const Codes& x) {
+#pragma unroll
+      for (int u = 0; u < kUnits; ++u) {
+        const uint32_t sc = e4m3x2_to_h2(x.s[u]), s0 = __byte_perm(sc, sc, 0x1010), s1 = __byte_perm(sc, sc, 0x3232);
+        const uint32_t cw[4] = {x.c[u].x, x.c[u].y, x.c[u].z, x.c[u].w};
+        const int key = key0 + u * kKeyStep;
+        uint8_t* block = to + (unit >> 1) * (kTileKeys * 128);
+        uint4 o[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          uint32_t v[4];
+          e2m1x8_to_h2(cw[i], v);
+          const uint32_t sx = i < 2 ? s0 : s1;
+          o[i] = make_uint4(h2_mul(v[0], sx), h2_mul(v[1], sx), h2_mul(v[2], sx), h2_mul(v[3], sx));
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          // lanes of one key write their four chunks in orders turned by their block, so that the eight of a phase hit eight
+          const int turn = (i + (unit >> 1)) & 3;
+          const uint4 v = turn == 0 ? o[0] : turn == 1 ? o[1] : turn == 2 ? o[2] : o[3];
+          *reinterpret_cast<uint4*>(block + sw128_offset(key, (unit & 1) * 4 + turn)) = v;
+        }
+      }
+    };
+    auto publish = [&](uint64_t* bar) {
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar);
+    };
+    Codes kc, vc;
+    int pg[kUnits];
+    look_up(0);
+#pragma unroll
+    for (int u = 0; u < kUnits; ++u) pg[u] = page[u];
+    ask(a.c.k, a.c.k_scales, 0, pg, kc);
+    bool ok = true;
+    for (int t = 0; t < nt && ok; ++t) {
+      // K(t): its codes are here or on their way; V(t)'s are asked for, the next tile's pages looked up
+      ask(a.c.v, a.c.v_scales, t, pg, vc);
+      look_up(t + 1);
+      if (w < 4) bad_keys[(t + 2) % kTileMarks][w] = 0, nan_keys[(t + 2) % kTileMarks][w] = 0;  // (used last six tiles ago)
+      if (unit == 0) {
+#pragma unroll
+        for (int u = 0; u < kUnits; ++u) {
+          const int key = key0 + u * kKeyStep, pos = (t0 + t) * kTileKeys + key;
+          if (pos < keys && (pg[u] < 1 || pg[u] > a.c.pages)) {
+            dev_fail(a.err, kDevBadPage);
+            atomicOr(&bad_keys[t % kTileMarks][key >> 5], 1u << (key & 31));
+          }
+        }
+      }
+      ok = t == 0 || wait(&qk_done[(t - 1) & 1], (t - 1) >> 1, kDevWaitEmpty);
+      if (!ok) break;
+      convert(ks, kc);
+      publish(&k_full);
+      // V(t)
+      if ((t0 + t + 1) * kTileKeys > all_see) {  // a masked tile: NaN must not meet the zero probabilities of rows that do not see it
+#pragma unroll
+        for (int u = 0; u < kUnits; ++u)
+          if ((vc.s[u] & 0x7f) == 0x7f || (vc.s[u] & 0x7f00) == 0x7f00) {
+            const int key = key0 + u * kKeyStep;
+            atomicOr(&nan_keys[t % kTileMarks][key >> 5], 1u << (key & 31));
+            vc.s[u] = 0;
+          }
+      }
+#pragma unroll
+      for (int u = 0; u < kUnits; ++u) pg[u] = page[u];
+      if (t + 1 < nt) ask(a.c.k, a.c.k_scales, t + 1, pg, kc);
+      ok = wait(&pv_done, t - 1, kDevWaitEmpty);
+      if (!ok) break;
+      convert(vs, vc);
+      publish(&v_full);
+    }
+  } else {
+    // ---------------------------------------------------------------- the softmax
+    const int f = f0 + tid, i_row = f / G;
+    const bool real = f < R;
+    const float coef = fabsf(a.scale) * a.c.k_scale * kLog2e * q_inv[tid];
+    const uint32_t see = !real ? 0u : a.b.anc ? a.b.anc[sq.row0 + i_row] : 0u;
+    const int limit = real ? sq.pos + i_row + 1 : 0;  // (no masks) positions this row sees
+    const uint32_t lane_addr = tmem + (uint32_t(warp * 32) << 16);
+    float m = -INFINITY, l = 0.f;
+    bool ok = true;
+    for (int t = 0; t < nt && ok; ++t) {
+      ok = wait(&qk_done[t & 1], t >> 1, kDevWaitTmemFull);
+      if (!ok) break;
+      tc_fence_after();
+      const uint32_t s_addr = lane_addr + uint32_t(t & 1) * kTileKeys;
+      const int base_pos = (t0 + t) * kTileKeys;
+      uint32_t bad = 0;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) bad |= bad_keys[t % kTileMarks][c];
+      const bool masked = base_pos + kTileKeys > all_see || bad;
+      if (masked && !(ok = wait(&pv_done, t - 1, kDevWaitTmemFull) && wait(&v_full, t, kDevWaitFull))) break;  // the marks of V's NaN (in order: a barrier tells the parity only)
+      // which of the 32 keys from c * 32 on this row sees
+      auto visible = [&](int c) {
+        const int p0 = base_pos + c * 32;
+        uint32_t bits;
+        if (a.b.anc) {  // the context, then the row's ancestors
+          const int ctx = sq.pos - p0;  // keys of the context among them
+          const uint32_t in = ctx >= 32 ? 0xffffffffu : ctx <= 0 ? 0u : (1u << ctx) - 1u;
+          const uint32_t mine = sq.n >= 32 ? see : see & ((1u << sq.n) - 1u);
+          bits = in | (ctx >= 32 ? 0u : ctx >= 0 ? mine << ctx : ctx > -32 ? mine >> -ctx : 0u);
+        } else {
+          const int n = limit - p0;
+          bits = n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u;
+        }
+        return bits & ~bad_keys[t % kTileMarks][c];
+      };
+      float mx = -INFINITY;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        uint32_t v[32];
+        tmem_ld32(s_addr + c * 32, v);
+        tmem_ld_wait();
+        if (masked) {
+          const uint32_t vis = visible(c);
+#pragma unroll
+          for (int j = 0; j < 32; ++j) mx = fmaxf(mx, vis >> j & 1u ? __uint_as_float(v[j]) : -INFINITY);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) mx = fmaxf(mx, __uint_as_float(v[j]));
+        }
+      }
+      ok = wait(&pv_done, t - 1, kDevWaitTmemFull);  // P is read, O complete
+      if (!ok) break;
+      tc_fence_after();
+      const float top = mx * coef;  // (-inf where nothing is seen)
+      const bool grow = top > m + kLazy;
+      if (__any_sync(0xffffffffu, grow)) {
+        const float m_new = grow ? top : m, keep = m == -INFINITY ? 0.f : ex2(m - m_new);
+        l *= keep, m = m_new;
+        if (t > 0) {
+#pragma unroll 1
+          for (int c = 0; c < D / 32; ++c) {
+            uint32_t v[32];
+            tmem_ld32(lane_addr + kOcol + c * 32, v);
+            tmem_ld_wait();
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(__uint_as_float(v[j]) * keep);
+            tmem_st32(lane_addr + kOcol + c * 32, v);
+          }
+          tmem_st_wait();
+        }
+      }
+      const float base = m == -INFINITY ? 0.f : m - kPShift;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        uint32_t v[32];
+        tmem_ld32(s_addr + c * 32, v);
+        tmem_ld_wait();
+        uint32_t vis = 0xffffffffu, nan = 0;
+        if (masked) vis = visible(c), nan = nan_keys[t % kTileMarks][c] & vis;
+        float p[32];
+#pragma unroll
+        for (int j = 0; j < 32; ++j) {
+          p[j] = ex2(fmaf(__uint_as_float(v[j]), coef, -base));
+          if (masked) p[j] = vis >> j & 1u ? p[j] : 0.f;
+        }
+#pragma unroll
+        for (int j = 0; j < 32; j += 4) l += (p[j] + p[j + 1]) + (p[j + 2] + p[j + 3]);
+        if (nan) {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) p[j] = nan >> j & 1u ? NAN : p[j];
+        }
+        uint8_t* to = ps + (c >> 1) * (kTileRows * 128);
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+          *reinterpret_cast<uint4*>(to + sw128_offset(tid, (c & 1) * 4 + x)) =
+              make_uint4(h2(p[8 * x], p[8 * x + 1]), h2(p[8 * x + 2], p[8 * x + 3]), h2(p[8 * x + 4], p[8 * x + 5]), h2(p[8 * x + 6], p[8 * x + 7]));
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&p_full);
+    }
+    // ---- the result
+    if (ok && wait(&pv_done, nt - 1, kDevWaitTmemFull)) {
+      tc_fence_after();
+      const bool empty = m == -INFINITY && l == 0.f;
+      const float scale = empty ? 0.f : a.c.v_scale / l;
+      const int row = sq.row0 + (real ? i_row : 0), head = h * G + (real ? f % G : 0);
+      T* to = static_cast<T*>(a.out.p) + row * a.out.row + head * a.out.head;
+#pragma unroll 1
+      for (int c = 0; c < D / 32; ++c) {
+        uint32_t v[32];
+        tmem_ld32(lane_addr + kOcol + c * 32, v);
+        tmem_ld_wait();
+        if (!real) continue;
+        if (splits > 1) {
+#pragma unroll
+          for (int j = 0; j < 32; j += 4) *reinterpret_cast<uint4*>(part + size_t(tid) * D + c * 32 + j) = make_uint4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+        } else if (a.out_vec) {
+#pragma unroll
+          for (int j = 0; j < 32; j += 8) {
+            T e[8];
+#pragma unroll
+            for (int x = 0; x < 8; ++x) e[x] = from_f32<T>(empty ? 0.f : __uint_as_float(v[j + x]) * scale);
+            *reinterpret_cast<uint4*>(to + c * 32 + j) = *reinterpret_cast<const uint4*>(e);
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) to[c * 32 + j] = from_f32<T>(empty ? 0.f : __uint_as_float(v[j]) * scale);
+        }
+      }
+      if (splits > 1) part[kTileRows * D + tid] = m, part[kTileRows * D + kTileRows + tid] = l;
+      else if (real && a.lse) a.lse[size_t(row) * a.q_heads + head] = empty ? -INFINITY : (m + log2f(l) - kPShift) * kLn2;
+    }
+    tc_fence_before();
+  }
+  __syncthreads();
+  if (warp == 12) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+  }
+}
+
+// The splits' partial results of the tile kernel: a warp a query row, in the order of the splits.
+template <typename T, int D>
+__global__ void __launch_bounds__(256) kv4_tile_join_kernel(AttnArgs a, int splits) {
+  pdl_sync();  // first statement: see common.cuh
+  const int lane = threadIdx.x & 31, G = a.q_heads / a.c.kv_heads, H = a.c.kv_heads, h = blockIdx.y;
+  const int r = blockIdx.x * 8 + (threadIdx.x >> 5);  // packed row * G + head of the group
+  const int row = r / G, head = h * G + r % G;
+  if (row >= a.b.rows) return;
+  // the sequence and its first tile
+  int before = 0, seq = -1, tile0 = 0;
+  for (int s0 = 0; s0 < a.b.seqs && seq < 0; s0 += 32) {
+    const int s = s0 + lane;
+    Kv4Seq q{0, 0, 0, 0, false};
+    if (s < a.b.seqs) q = kv4_seq(a.c, a.b, s);
+    const int n = q.ok ? (q.n * G + kTileRows - 1) / kTileRows : 0;
+    int end = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, end, o);
+      if (lane >= o) end += v;
+    }
+    end += before;
+    const unsigned mine = __ballot_sync(0xffffffffu, q.ok && row >= q.row0 && row < q.row0 + q.n);
+    if (mine) {
+      seq = s0 + __ffs(mine) - 1;
+      tile0 = __shfl_sync(0xffffffffu, end - n, __ffs(mine) - 1);
+    }
+    before = __shfl_sync(0xffffffffu, end, 31);
+  }
+  if (seq < 0) return;
+  const int f = (row - a.b.row0[seq]) * G + r % G, in = f % kTileRows;
+  const float* parts = a.parts + (size_t(tile0 + f / kTileRows) * H + h) * splits * tile_part_floats(D);
+  float mm = -INFINITY;
+  for (int s = 0; s < splits; ++s) mm = fmaxf(mm, parts[s * tile_part_floats(D) + kTileRows * D + in]);
+  float l = 0.f, o[D / 32] = {};
+  for (int s = 0; s < splits; ++s) {
+    const float* p = parts + s * tile_part_floats(D);
+    const float ps = p[kTileRows * D + kTileRows + in], w = part_weight(p[kTileRows * D + in], ps, mm);
+    if (w == 0.f) continue;  // (a split without keys has written no O)
+    l = fmaf(ps, w, l);
+#pragma unroll
+    for (int j = 0; j < D / 32; ++j) o[j] = fmaf(p[size_t(in) * D + j * 32 + lane], w, o[j]);
+  }
+  const bool empty = mm == -INFINITY && l == 0.f;
+  T* to = static_cast<T*>(a.out.p) + row * a.out.row + head * a.out.head;
+#pragma unroll
+  for (int j = 0; j < D / 32; ++j) to[j * 32 + lane] = from_f32<T>(empty ? 0.f : o[j] / l * a.c.v_scale);
+  if (a.lse && lane == 0) a.lse[size_t(row) * a.q_heads + head] = empty ? -INFINITY : (mm + log2f(l) - kPShift) * kLn2;
+}
+
 template <typename T, int D>
 int decode_init() {
   LB_CUDA(cudaFuncSetAttribute(kv4_decode_kernel<T, D, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, dec_smem(D)));
+  LB_CUDA(cudaFuncSetAttribute(kv4_tile_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, TileSmem<D>::kBytes));
   LB_CUDA(cudaFuncSetAttribute(kv4_decode_kernel<T, D, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, dec_smem(D)));
   return LING_B200_OK;
 }
@@ -765,6 +1254,43 @@ int decode_launch(const AttnArgs& a, int sms, cudaStream_t s) {
                                : decode_launch_t<T, 256>(a, solo, sms, s);
 }
 
+// How a batch with up to these rows and positions runs.  Up to kDecodeRows query rows of a kv head the decode kernel reads the cache once
+// per 8 of them; beyond, the tile kernel once per 128, contexts split over CTAs where the row tiles alone do not fill the device.
+constexpr int kDecodeRows = 16, kTileCtas = 148, kTileSplitKeys = 512;  // CTAs wanted; positions that a split is worth
+struct Plan {
+  bool tile = false, solo = false;
+  int row_tiles = 0, splits = 1;
+};
+Plan make_plan(const ling_b200_kv4& c, const ling_b200_kv4_batch& b, int q_heads) {
+  Plan p;
+  const int G = q_heads / c.kv_heads;
+  p.tile = (long long)b.max_rows * G > kDecodeRows;
+  if (!p.tile) {
+    p.solo = decode_solo(c, b, q_heads);
+    return p;
+  }
+  const long long most = (long long)b.seqs * (((long long)b.max_rows * G + kTileRows - 1) / kTileRows), packed = (long long)b.rows * G / kTileRows + b.seqs;
+  p.row_tiles = int(std::min(most, packed));
+  p.splits = int(std::max(1ll, std::min<long long>(kTileCtas / ((long long)p.row_tiles * c.kv_heads), (b.max_context + kTileSplitKeys - 1) / kTileSplitKeys)));
+  return p;
+}
+template <typename T, int D>
+int tile_launch_t(const AttnArgs& a, const Plan& p, cudaStream_t s) {
+  LB_CUDA(launch_kernel(kv4_tile_kernel<T, D>, dim3(p.row_tiles, a.c.kv_heads, p.splits), dim3(kTileThreads), size_t(TileSmem<D>::kBytes), s, a, p.splits));
+  LB_LAUNCH("kv4_tile_kernel");
+  if (p.splits > 1) {
+    LB_CUDA(launch_dependent(kv4_tile_join_kernel<T, D>, dim3(ceil_div(a.b.rows * (a.q_heads / a.c.kv_heads), 8), a.c.kv_heads), dim3(256), size_t(0), s, a, p.splits));
+    LB_LAUNCH("kv4_tile_join_kernel");
+  }
+  return LING_B200_OK;
+}
+template <typename T>
+int attention_launch(const AttnArgs& a, int sms, cudaStream_t s) {
+  const Plan p = make_plan(a.c, a.b, a.q_heads);
+  if (!p.tile) return decode_launch<T>(a, sms, s);
+  return a.c.head_dim == 64 ? tile_launch_t<T, 64>(a, p, s) : a.c.head_dim == 128 ? tile_launch_t<T, 128>(a, p, s) : tile_launch_t<T, 256>(a, p, s);
+}
+
 DeviceInfo g_devices[kMaxDevices];
 std::mutex g_mutex;
 
@@ -785,7 +1311,9 @@ using namespace lb::d4;
 extern "C" size_t ling_b200_kv4_attention_workspace(const ling_b200_kv4* cache, const ling_b200_kv4_batch* batch, int q_heads) {
   const char* who = "kv4_attention_workspace";
   if (!kv4_cache_ok(cache, who) || !kv4_batch_ok(cache, batch, who) || !heads_ok(cache, q_heads, who)) return 0;
-  return kJoinBytes + size_t(decode_solo(*cache, *batch, q_heads) ? kDecMaxWorkers : kDecMaxCtas) * 2 * dec_part_floats(cache->head_dim) * 4;
+  const Plan p = make_plan(*cache, *batch, q_heads);
+  if (p.tile) return kJoinBytes + (p.splits > 1 ? size_t(p.row_tiles) * cache->kv_heads * p.splits * tile_part_floats(cache->head_dim) * 4 : 0);
+  return kJoinBytes + size_t(p.solo ? kDecMaxWorkers : kDecMaxCtas) * 2 * dec_part_floats(cache->head_dim) * 4;
 }
 
 extern "C" int ling_b200_kv4_attention(int device, const ling_b200_kv4* cache, const ling_b200_kv4_batch* batch, int type,
@@ -804,7 +1332,7 @@ extern "C" int ling_b200_kv4_attention(int device, const ling_b200_kv4* cache, c
     return LING_B200_ERR_ARG;
   }
   const long long tiles = ((long long)batch->max_rows * (q_heads / cache->kv_heads) + kDecRows - 1) / kDecRows * cache->kv_heads;
-  if (tiles * batch->seqs > (1ll << 30) / (batch->max_context / 16 + 1)) {
+  if (!make_plan(*cache, *batch, q_heads).tile && tiles * batch->seqs > (1ll << 30) / (batch->max_context / 16 + 1)) {
     set_error("kv4_attention: the batch's bounds (seqs x max_rows x max_context) are beyond 2^30 steps of the kernel");
     return LING_B200_ERR_UNSUPPORTED;
   }
@@ -818,8 +1346,7 @@ extern "C" int ling_b200_kv4_attention(int device, const ling_b200_kv4* cache, c
   int sms = 0;
   if (const int r = enter_device(guard, device, g_devices, g_mutex, attention_init, &sms)) return r;
   AttnArgs a{*cache, *batch, *q, *out, q_heads, scale, lse, err, static_cast<Join*>(workspace),
-             reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + kJoinBytes), false};
-  a.q_vec = rows_vec(*q, type);
+             reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + kJoinBytes), rows_vec(*q, type), rows_vec(*out, type)};
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  return type == LING_B200_BF16 ? decode_launch<__nv_bfloat16>(a, sms, s) : decode_launch<__half>(a, sms, s);
+  return type == LING_B200_BF16 ? attention_launch<__nv_bfloat16>(a, sms, s) : attention_launch<__half>(a, sms, s);
 }
