@@ -728,17 +728,17 @@ __global__ void __launch_bounds__(kJoinThreads) kv4_join_kernel(AttnArgs a) {
 // ---------------------------------------------------------------------------------------------- many query rows
 // The tile kernel: 128 query rows of one (sequence, kv head) against its keys, 128 at a time, on tcgen05.mma kind::f16 with the
 // accumulators in TMEM.  Roles:
-//   warps 4..11  turn a tile's codes into FP16 operands in 128B-swizzled shared memory, keys as rows: K as the score product's
-//                K-major B operand, V, in the same layout, as the value product's MN-major one (no transposition).  Their
-//                loads run one tile ahead in registers, the page ids two.
-//   warp 12      one thread issues the MMAs: S(t+1) = Q K(t+1)^T before O += P(t) V(t), S double in TMEM, so that the tensor
-//                core works while the softmax of the tile in between runs.
-//   warps 0..3   a thread a row (its TMEM lane): maximum, probabilities to FP16 in shared memory, sum; O is scaled in TMEM only when
-//                a score exceeds the row's reference by 2^kLazy.
+//   warps 8..15  turn a tile's codes into FP16 operands in 128B-swizzled shared memory, keys as rows: K as the score product's
+//                K-major B operand, V, in the same layout, as the value product's MN-major one (no transposition).  K(t+1) comes
+//                before V(t), so that S(t+1) = Q K(t+1)^T runs under the softmax of tile t.  Loads run ahead in registers.
+//   warp 16      one thread issues the MMAs: S(t+1), double in TMEM, then O += P(t) V(t).
+//   warps 0..7   a thread half a row (its TMEM lane, 64 of the tile's keys): maximum, probabilities to FP16 in shared memory, sum; O
+//                is scaled in TMEM only when a score exceeds the row's reference by 2^kLazy.
 // What bounds it is shared memory: operands are read once by the MMAs and written once by the converting warps (D = 256: 224 KB
 // and 160 KB a tile, 3072 cycles at 128 bytes, against 2048 cycles of MMA).
 // Every wait is bounded; one that runs out is recorded and the CTA leaves with its TMEM freed.
-constexpr int kTileRows = 128, kTileKeys = 128, kTileThreads = 13 * 32, kTileWorkers = 256, kTileMarks = 8;
+constexpr int kTileRows = 128, kTileKeys = 128, kTileWarps = 17, kTileThreads = kTileWarps * 32, kTileWorkers = 256, kTileMarks = 8;
+constexpr int kMmaWarp = 16;
 template <int D>
 struct TileSmem {
   static constexpr int kOperand = 256 * D;  // 128 rows of D halves: [D / 64][128][128 B]
@@ -766,7 +766,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv4_tile_kernel(AttnArgs a, i
   uint8_t* ps = vs + kOperand;
   __shared__ uint64_t k_full, v_full, qk_done[2], p_full, pv_done;  // (two score barriers: the next tile's may be done before this one's is waited for)
   __shared__ uint32_t tmem_slot, bad_keys[kTileMarks][4], nan_keys[kTileMarks][4];  // by tile: keys on bad pages; (masked tiles) keys whose V is NaN
-  __shared__ float q_inv[kTileRows];
+  __shared__ float q_inv[kTileRows], row_max[2][kTileRows];  // (by half; at the end the sums)
   __shared__ int where[2];
   __shared__ volatile int failed;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -805,7 +805,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv4_tile_kernel(AttnArgs a, i
     mbar_init(&v_full, kTileWorkers / 32);
     mbar_init(&qk_done[0], 1);
     mbar_init(&qk_done[1], 1);
-    mbar_init(&p_full, 4);
+    mbar_init(&p_full, 8);
     mbar_init(&pv_done, 1);
     failed = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -825,7 +825,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv4_tile_kernel(AttnArgs a, i
     if (tid < kTileRows) part[kTileRows * D + tid] = -INFINITY, part[kTileRows * D + kTileRows + tid] = 0.f;
     return;
   }
-  if (warp == 12) {
+  if (warp == kMmaWarp) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(512) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     tc_fence_before();
@@ -835,7 +835,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv4_tile_kernel(AttnArgs a, i
   {
     constexpr int kLanes = D / 8, kRowsAtOnce = 32 / kLanes, kFly = 4;
     const int sub = lane / kLanes, piece = lane % kLanes;
-    for (int r0 = warp * kRowsAtOnce * kFly; r0 < kTileRows; r0 += 13 * kRowsAtOnce * kFly) {
+    for (int r0 = warp * kRowsAtOnce * kFly; r0 < kTileRows; r0 += kTileWarps * kRowsAtOnce * kFly) {
       uint4 w[kFly];
 #pragma unroll
       for (int i = 0; i < kFly; ++i) {
@@ -886,7 +886,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv4_tile_kernel(AttnArgs a, i
     return false;
   };
 
-  if (warp == 12) {
+  if (warp == kMmaWarp) {
     // ---------------------------------------------------------------- the MMAs
     if (lane == 0) {
       constexpr uint32_t kIdescS = umma_idesc_f16(kTileKeys), kIdescO = umma_idesc_f16(D) | 1u << 16;  // (bit 16: B is MN-major)
@@ -916,21 +916,21 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv4_tile_kernel(AttnArgs a, i
       }
     }
     __syncwarp();
-  } else if (warp >= 4) {
+  } else if (warp >= 8) {
     // ---------------------------------------------------------------- the operands
-    const int w = tid - 128, unit = w % (D / 32), key0 = w / (D / 32);  // units of 32 dims: keys key0, key0 + 256 / (D / 32), ..
-    constexpr int kKeyStep = kTileWorkers / (D / 32);
+    // a worker's units of 32 dims: eight neighbouring lanes take eight keys (their stores hit eight different chunks)
+    constexpr int kPer = D / 32, kKeyStep = kTileWorkers / kPer;
+    const int w = tid - 256, unit = (w >> 3) % kPer, key0 = (w >> 3) / kPer * 8 + (w & 7);  // keys key0, key0 + kKeyStep, ..
     const int* table = a.c.tables + size_t(sq.slot) * a.c.max_pages;
     struct Codes {
       uint4 c[kUnits];
       uint16_t s[kUnits];
     };
-    int page[kUnits];  // of the tile after the one whose codes are asked for
-    auto look_up = [&](int t) {
+    auto look_up = [&](int t, int (&pg)[kUnits]) {
 #pragma unroll
       for (int u = 0; u < kUnits; ++u) {
         const int pos = (t0 + t) * kTileKeys + key0 + u * kKeyStep;
-        page[u] = t < nt && pos < keys ? table[pos >> lp] : -1;
+        pg[u] = t < nt && pos < keys ? table[pos >> lp] : -1;
       }
     };
     auto ask = [&](const uint8_t* codes, const uint8_t* scales, int t, const int (&pg)[kUnits], Codes& x) {
@@ -952,20 +952,12 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv4_tile_kernel(AttnArgs a, i
         const uint32_t cw[4] = {x.c[u].x, x.c[u].y, x.c[u].z, x.c[u].w};
         const int key = key0 + u * kKeyStep;
         uint8_t* block = to + (unit >> 1) * (kTileKeys * 128);
-        uint4 o[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           uint32_t v[4];
           e2m1x8_to_h2(cw[i], v);
           const uint32_t sx = i < 2 ? s0 : s1;
-          o[i] = make_uint4(h2_mul(v[0], sx), h2_mul(v[1], sx), h2_mul(v[2], sx), h2_mul(v[3], sx));
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          // lanes of one key write their four chunks in orders turned by their block, so that the eight of a phase hit eight
-          const int turn = (i + (unit >> 1)) & 3;
-          const uint4 v = turn == 0 ? o[0] : turn == 1 ? o[1] : turn == 2 ? o[2] : o[3];
-          *reinterpret_cast<uint4*>(block + sw128_offset(key, (unit & 1) * 4 + turn)) = v;
+          *reinterpret_cast<uint4*>(block + sw128_offset(key, (unit & 1) * 4 + i)) = make_uint4(h2_mul(v[0], sx), h2_mul(v[1], sx), h2_mul(v[2], sx), h2_mul(v[3], sx));
         }
       }
     };
@@ -974,33 +966,39 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv4_tile_kernel(AttnArgs a, i
       __syncwarp();
       if (lane == 0) mbar_arrive(bar);
     };
-    Codes kc, vc;
-    int pg[kUnits];
-    look_up(0);
+    auto mark_bad = [&](int t, const int (&pg)[kUnits]) {
+      if (unit != 0) return;
 #pragma unroll
-    for (int u = 0; u < kUnits; ++u) pg[u] = page[u];
-    ask(a.c.k, a.c.k_scales, 0, pg, kc);
-    bool ok = true;
-    for (int t = 0; t < nt && ok; ++t) {
-      // K(t): its codes are here or on their way; V(t)'s are asked for, the next tile's pages looked up
-      ask(a.c.v, a.c.v_scales, t, pg, vc);
-      look_up(t + 1);
-      if (w < 4) bad_keys[(t + 2) % kTileMarks][w] = 0, nan_keys[(t + 2) % kTileMarks][w] = 0;  // (used last six tiles ago)
-      if (unit == 0) {
-#pragma unroll
-        for (int u = 0; u < kUnits; ++u) {
-          const int key = key0 + u * kKeyStep, pos = (t0 + t) * kTileKeys + key;
-          if (pos < keys && (pg[u] < 1 || pg[u] > a.c.pages)) {
-            dev_fail(a.err, kDevBadPage);
-            atomicOr(&bad_keys[t % kTileMarks][key >> 5], 1u << (key & 31));
-          }
+      for (int u = 0; u < kUnits; ++u) {
+        const int key = key0 + u * kKeyStep, pos = (t0 + t) * kTileKeys + key;
+        if (t < nt && pos < keys && (pg[u] < 1 || pg[u] > a.c.pages)) {
+          dev_fail(a.err, kDevBadPage);
+          atomicOr(&bad_keys[t % kTileMarks][key >> 5], 1u << (key & 31));
         }
       }
-      ok = t == 0 || wait(&qk_done[(t - 1) & 1], (t - 1) >> 1, kDevWaitEmpty);
-      if (!ok) break;
-      convert(ks, kc);
-      publish(&k_full);
-      // V(t)
+    };
+    Codes kc, vc;
+    int pg[3][kUnits];  // pages of tiles t, t + 1, t + 2
+    look_up(0, pg[0]);
+    look_up(1, pg[1]);
+    ask(a.c.k, a.c.k_scales, 0, pg[0], kc);
+    mark_bad(0, pg[0]);
+    convert(ks, kc);
+    publish(&k_full);
+    ask(a.c.k, a.c.k_scales, 1, pg[1], kc);
+    bool ok = true;
+    for (int t = 0; t < nt && ok; ++t) {
+      ask(a.c.v, a.c.v_scales, t, pg[0], vc);
+      look_up(t + 2, pg[2]);
+      if (w < 4) bad_keys[(t + 3) % kTileMarks][w] = 0, nan_keys[(t + 3) % kTileMarks][w] = 0;  // (last used five tiles ago)
+      if (t + 1 < nt) {  // K(t + 1), where K(t) was
+        ok = wait(&qk_done[t & 1], t >> 1, kDevWaitEmpty);
+        if (!ok) break;
+        mark_bad(t + 1, pg[1]);
+        convert(ks, kc);
+        publish(&k_full);
+      }
+      ask(a.c.k, a.c.k_scales, t + 2, pg[2], kc);
       if ((t0 + t + 1) * kTileKeys > all_see) {  // a masked tile: NaN must not meet the zero probabilities of rows that do not see it
 #pragma unroll
         for (int u = 0; u < kUnits; ++u)
@@ -1010,110 +1008,113 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv4_tile_kernel(AttnArgs a, i
             vc.s[u] = 0;
           }
       }
-#pragma unroll
-      for (int u = 0; u < kUnits; ++u) pg[u] = page[u];
-      if (t + 1 < nt) ask(a.c.k, a.c.k_scales, t + 1, pg, kc);
-      ok = wait(&pv_done, t - 1, kDevWaitEmpty);
+      ok = wait(&pv_done, t - 1, kDevWaitEmpty);  // V(t), where V(t - 1) was
       if (!ok) break;
       convert(vs, vc);
       publish(&v_full);
+#pragma unroll
+      for (int u = 0; u < kUnits; ++u) pg[0][u] = pg[1][u], pg[1][u] = pg[2][u];
     }
   } else {
     // ---------------------------------------------------------------- the softmax
-    const int f = f0 + tid, i_row = f / G;
+    const int r = tid & (kTileRows - 1), half = tid >> 7, f = f0 + r, i_row = f / G;  // row r, keys half * 64 .. + 64 of a tile
     const bool real = f < R;
-    const float coef = fabsf(a.scale) * a.c.k_scale * kLog2e * q_inv[tid];
-    const uint32_t see = !real ? 0u : a.b.anc ? a.b.anc[sq.row0 + i_row] : 0u;
+    const float coef = fabsf(a.scale) * a.c.k_scale * kLog2e * q_inv[r];
+    const uint32_t see = real && a.b.anc ? a.b.anc[sq.row0 + i_row] : 0u;
     const int limit = real ? sq.pos + i_row + 1 : 0;  // (no masks) positions this row sees
-    const uint32_t lane_addr = tmem + (uint32_t(warp * 32) << 16);
+    const uint32_t lane_addr = tmem + (uint32_t((warp & 3) * 32) << 16);
     float m = -INFINITY, l = 0.f;
     bool ok = true;
     for (int t = 0; t < nt && ok; ++t) {
       ok = wait(&qk_done[t & 1], t >> 1, kDevWaitTmemFull);
-      if (!ok) break;
-      tc_fence_after();
-      const uint32_t s_addr = lane_addr + uint32_t(t & 1) * kTileKeys;
-      const int base_pos = (t0 + t) * kTileKeys;
+      if (ok) tc_fence_after();
+      const uint32_t s_addr = lane_addr + uint32_t(t & 1) * kTileKeys + half * 64;
+      const int base_pos = (t0 + t) * kTileKeys + half * 64;
       uint32_t bad = 0;
 #pragma unroll
       for (int c = 0; c < 4; ++c) bad |= bad_keys[t % kTileMarks][c];
-      const bool masked = base_pos + kTileKeys > all_see || bad;
-      if (masked && !(ok = wait(&pv_done, t - 1, kDevWaitTmemFull) && wait(&v_full, t, kDevWaitFull))) break;  // the marks of V's NaN (in order: a barrier tells the parity only)
-      // which of the 32 keys from c * 32 on this row sees
-      auto visible = [&](int c) {
-        const int p0 = base_pos + c * 32;
-        uint32_t bits;
-        if (a.b.anc) {  // the context, then the row's ancestors
-          const int ctx = sq.pos - p0;  // keys of the context among them
-          const uint32_t in = ctx >= 32 ? 0xffffffffu : ctx <= 0 ? 0u : (1u << ctx) - 1u;
-          const uint32_t mine = sq.n >= 32 ? see : see & ((1u << sq.n) - 1u);
-          bits = in | (ctx >= 32 ? 0u : ctx >= 0 ? mine << ctx : ctx > -32 ? mine >> -ctx : 0u);
-        } else {
-          const int n = limit - p0;
-          bits = n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u;
+      const bool masked = (t0 + t + 1) * kTileKeys > all_see || bad;
+      uint32_t vis[2] = {0xffffffffu, 0xffffffffu};  // which of its 64 keys this row sees
+      if (masked) {
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const int p0 = base_pos + c * 32;
+          if (a.b.anc) {  // the context, then the row's ancestors
+            const int ctx = sq.pos - p0;  // keys of the context among them
+            const uint32_t mine = sq.n >= 32 ? see : see & ((1u << sq.n) - 1u);
+            vis[c] = ctx >= 32 ? 0xffffffffu : ctx >= 0 ? (1u << ctx) - 1u | mine << ctx : ctx > -32 ? mine >> -ctx : 0u;
+          } else {
+            const int n = limit - p0;
+            vis[c] = n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u;
+          }
+          vis[c] &= ~bad_keys[t % kTileMarks][half * 2 + c];
         }
-        return bits & ~bad_keys[t % kTileMarks][c];
-      };
+      }
       float mx = -INFINITY;
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
+      for (int c = 0; c < 2; ++c) {
         uint32_t v[32];
         tmem_ld32(s_addr + c * 32, v);
         tmem_ld_wait();
         if (masked) {
-          const uint32_t vis = visible(c);
 #pragma unroll
-          for (int j = 0; j < 32; ++j) mx = fmaxf(mx, vis >> j & 1u ? __uint_as_float(v[j]) : -INFINITY);
+          for (int j = 0; j < 32; ++j) mx = fmaxf(mx, vis[c] >> j & 1u ? __uint_as_float(v[j]) : -INFINITY);
         } else {
 #pragma unroll
           for (int j = 0; j < 32; ++j) mx = fmaxf(mx, __uint_as_float(v[j]));
         }
       }
-      ok = wait(&pv_done, t - 1, kDevWaitTmemFull);  // P is read, O complete
-      if (!ok) break;
+      row_max[half][r] = mx;
+      asm volatile("bar.sync 1, 256;" ::: "memory");  // the other half's maximum
+      mx = fmaxf(mx, row_max[half ^ 1][r]);
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+      ok = ok && wait(&pv_done, t - 1, kDevWaitTmemFull);              // P is read, O complete
+      if (masked) ok = ok && wait(&v_full, t, kDevWaitFull);           // the marks of V's NaN
       tc_fence_after();
       const float top = mx * coef;  // (-inf where nothing is seen)
       const bool grow = top > m + kLazy;
-      if (__any_sync(0xffffffffu, grow)) {
+      if (ok && __any_sync(0xffffffffu, grow)) {
         const float m_new = grow ? top : m, keep = m == -INFINITY ? 0.f : ex2(m - m_new);
         l *= keep, m = m_new;
         if (t > 0) {
 #pragma unroll 1
-          for (int c = 0; c < D / 32; ++c) {
-            uint32_t v[32];
-            tmem_ld32(lane_addr + kOcol + c * 32, v);
+          for (int c = half * (D / 64); c < (half + 1) * (D / 64); ++c) {
+            uint32_t x[32];
+            tmem_ld32(lane_addr + kOcol + c * 32, x);
             tmem_ld_wait();
 #pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(__uint_as_float(v[j]) * keep);
-            tmem_st32(lane_addr + kOcol + c * 32, v);
+            for (int j = 0; j < 32; ++j) x[j] = __float_as_uint(__uint_as_float(x[j]) * keep);
+            tmem_st32(lane_addr + kOcol + c * 32, x);
           }
           tmem_st_wait();
         }
       }
       const float base = m == -INFINITY ? 0.f : m - kPShift;
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
+      for (int c = 0; c < 2; ++c) {
         uint32_t v[32];
         tmem_ld32(s_addr + c * 32, v);
         tmem_ld_wait();
-        uint32_t vis = 0xffffffffu, nan = 0;
-        if (masked) vis = visible(c), nan = nan_keys[t % kTileMarks][c] & vis;
         float p[32];
 #pragma unroll
-        for (int j = 0; j < 32; ++j) {
-          p[j] = ex2(fmaf(__uint_as_float(v[j]), coef, -base));
-          if (masked) p[j] = vis >> j & 1u ? p[j] : 0.f;
+        for (int j = 0; j < 32; ++j) p[j] = ex2(fmaf(__uint_as_float(v[j]), coef, -base));
+        if (masked) {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) p[j] = vis[c] >> j & 1u ? p[j] : 0.f;
         }
 #pragma unroll
         for (int j = 0; j < 32; j += 4) l += (p[j] + p[j + 1]) + (p[j + 2] + p[j + 3]);
-        if (nan) {
+        if (masked) {
+          const uint32_t nan = nan_keys[t % kTileMarks][half * 2 + c] & vis[c];
+          if (nan) {
 #pragma unroll
-          for (int j = 0; j < 32; ++j) p[j] = nan >> j & 1u ? NAN : p[j];
+            for (int j = 0; j < 32; ++j) p[j] = nan >> j & 1u ? NAN : p[j];
+          }
         }
-        uint8_t* to = ps + (c >> 1) * (kTileRows * 128);
+        uint8_t* to = ps + half * (kTileRows * 128);
 #pragma unroll
         for (int x = 0; x < 4; ++x)
-          *reinterpret_cast<uint4*>(to + sw128_offset(tid, (c & 1) * 4 + x)) =
+          *reinterpret_cast<uint4*>(to + sw128_offset(r, c * 4 + x)) =
               make_uint4(h2(p[8 * x], p[8 * x + 1]), h2(p[8 * x + 2], p[8 * x + 3]), h2(p[8 * x + 4], p[8 * x + 5]), h2(p[8 * x + 6], p[8 * x + 7]));
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -1121,7 +1122,10 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv4_tile_kernel(AttnArgs a, i
       __syncwarp();
       if (lane == 0) mbar_arrive(&p_full);
     }
-    // ---- the result
+    // ---- the result, half of the dims a thread
+    row_max[half][r] = l;
+    asm volatile("bar.sync 1, 256;" ::: "memory");
+    l = row_max[0][r] + row_max[1][r];
     if (ok && wait(&pv_done, nt - 1, kDevWaitTmemFull)) {
       tc_fence_after();
       const bool empty = m == -INFINITY && l == 0.f;
@@ -1129,34 +1133,36 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv4_tile_kernel(AttnArgs a, i
       const int row = sq.row0 + (real ? i_row : 0), head = h * G + (real ? f % G : 0);
       T* to = static_cast<T*>(a.out.p) + row * a.out.row + head * a.out.head;
 #pragma unroll 1
-      for (int c = 0; c < D / 32; ++c) {
-        uint32_t v[32];
-        tmem_ld32(lane_addr + kOcol + c * 32, v);
+      for (int c = half * (D / 64); c < (half + 1) * (D / 64); ++c) {
+        uint32_t x[32];
+        tmem_ld32(lane_addr + kOcol + c * 32, x);
         tmem_ld_wait();
         if (!real) continue;
         if (splits > 1) {
 #pragma unroll
-          for (int j = 0; j < 32; j += 4) *reinterpret_cast<uint4*>(part + size_t(tid) * D + c * 32 + j) = make_uint4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+          for (int j = 0; j < 32; j += 4) *reinterpret_cast<uint4*>(part + size_t(r) * D + c * 32 + j) = make_uint4(x[j], x[j + 1], x[j + 2], x[j + 3]);
         } else if (a.out_vec) {
 #pragma unroll
           for (int j = 0; j < 32; j += 8) {
             T e[8];
 #pragma unroll
-            for (int x = 0; x < 8; ++x) e[x] = from_f32<T>(empty ? 0.f : __uint_as_float(v[j + x]) * scale);
+            for (int y = 0; y < 8; ++y) e[y] = from_f32<T>(empty ? 0.f : __uint_as_float(x[j + y]) * scale);
             *reinterpret_cast<uint4*>(to + c * 32 + j) = *reinterpret_cast<const uint4*>(e);
           }
         } else {
 #pragma unroll
-          for (int j = 0; j < 32; ++j) to[c * 32 + j] = from_f32<T>(empty ? 0.f : __uint_as_float(v[j]) * scale);
+          for (int j = 0; j < 32; ++j) to[c * 32 + j] = from_f32<T>(empty ? 0.f : __uint_as_float(x[j]) * scale);
         }
       }
-      if (splits > 1) part[kTileRows * D + tid] = m, part[kTileRows * D + kTileRows + tid] = l;
-      else if (real && a.lse) a.lse[size_t(row) * a.q_heads + head] = empty ? -INFINITY : (m + log2f(l) - kPShift) * kLn2;
+      if (half == 0) {
+        if (splits > 1) part[kTileRows * D + r] = m, part[kTileRows * D + kTileRows + r] = l;
+        else if (real && a.lse) a.lse[size_t(row) * a.q_heads + head] = empty ? -INFINITY : (m + log2f(l) - kPShift) * kLn2;
+      }
     }
     tc_fence_before();
   }
   __syncthreads();
-  if (warp == 12) {
+  if (warp == kMmaWarp) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
   }
