@@ -142,6 +142,20 @@ __device__ __forceinline__ uint32_t h2_mul(uint32_t a, uint32_t b) {
   const __half2 r = __hmul2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
   return *reinterpret_cast<const uint32_t*>(&r);
 }
+// Two fp32 operations an instruction.
+__device__ __forceinline__ uint64_t f2_pack(float lo, float hi) { return uint64_t(__float_as_uint(hi)) << 32 | __float_as_uint(lo); }
+__device__ __forceinline__ uint64_t f2_fma(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t f2_add(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ float f2_lo(uint64_t a) { return __uint_as_float(uint32_t(a)); }
+__device__ __forceinline__ float f2_hi(uint64_t a) { return __uint_as_float(uint32_t(a >> 32)); }
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -922,42 +936,52 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv4_tile_kernel(AttnArgs a, i
     constexpr int kPer = D / 32, kKeyStep = kTileWorkers / kPer;
     const int w = tid - 256, unit = (w >> 3) % kPer, key0 = (w >> 3) / kPer * 8 + (w & 7);  // keys key0, key0 + kKeyStep, ..
     const int* table = a.c.tables + size_t(sq.slot) * a.c.max_pages;
+    // Of a tile's units: where their vectors are (kNone: no key, kBad: no page), as indices among the cache's vectors.
+    constexpr uint32_t kNone = 0xffffffffu, kBad = 0xfffffffeu;
     struct Codes {
       uint4 c[kUnits];
       uint16_t s[kUnits];
     };
-    auto look_up = [&](int t, int (&pg)[kUnits]) {
+    auto look_up = [&](int t, int (&page)[kUnits]) {
 #pragma unroll
       for (int u = 0; u < kUnits; ++u) {
         const int pos = (t0 + t) * kTileKeys + key0 + u * kKeyStep;
-        pg[u] = t < nt && pos < keys ? table[pos >> lp] : -1;
+        page[u] = t < nt && pos < keys ? table[pos >> lp] : -1;
       }
     };
-    auto ask = [&](const uint8_t* codes, const uint8_t* scales, int t, const int (&pg)[kUnits], Codes& x) {
+    auto locate = [&](int t, const int (&page)[kUnits], uint32_t (&vec)[kUnits]) {
 #pragma unroll
       for (int u = 0; u < kUnits; ++u) {
         const int pos = (t0 + t) * kTileKeys + key0 + u * kKeyStep;
+        vec[u] = (((uint32_t(page[u]) * H + h) << lp) + (pos & ((1 << lp) - 1)));
+        if (page[u] < 1 || page[u] > a.c.pages) vec[u] = t < nt && pos < keys ? kBad : kNone;
+      }
+    };
+    const uint8_t *k_unit = a.c.k + unit * 16, *v_unit = a.c.v + unit * 16, *ks_unit = a.c.k_scales + unit * 2, *vs_unit = a.c.v_scales + unit * 2;
+    auto ask = [&](const uint8_t* codes, const uint8_t* scales, const uint32_t (&vec)[kUnits], Codes& x) {
+#pragma unroll
+      for (int u = 0; u < kUnits; ++u) {
         x.c[u] = make_uint4(0, 0, 0, 0), x.s[u] = 0;
-        if (pg[u] >= 1 && pg[u] <= a.c.pages) {
-          const size_t vec = ((size_t(pg[u]) * H + h) << lp) + (pos & ((1 << lp) - 1));
-          x.c[u] = *reinterpret_cast<const uint4*>(codes + vec * (D / 2) + unit * 16);
-          x.s[u] = *reinterpret_cast<const uint16_t*>(scales + vec * (D / 16) + unit * 2);
+        if (vec[u] < kBad) {
+          x.c[u] = *reinterpret_cast<const uint4*>(codes + size_t(vec[u]) * (D / 2));
+          x.s[u] = *reinterpret_cast<const uint16_t*>(scales + size_t(vec[u]) * (D / 16));
         }
       }
     };
+    uint32_t chunk_at[4];  // where the unit's four 16-byte chunks lie (the keys of a thread differ by multiples of 8: the swizzle is one)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) chunk_at[i] = (unit >> 1) * (kTileKeys * 128) + sw128_offset(key0, (unit & 1) * 4 + i);
     auto convert = [&](uint8_t* to, const Codes& x) {
 #pragma unroll
       for (int u = 0; u < kUnits; ++u) {
         const uint32_t sc = e4m3x2_to_h2(x.s[u]), s0 = __byte_perm(sc, sc, 0x1010), s1 = __byte_perm(sc, sc, 0x3232);
         const uint32_t cw[4] = {x.c[u].x, x.c[u].y, x.c[u].z, x.c[u].w};
-        const int key = key0 + u * kKeyStep;
-        uint8_t* block = to + (unit >> 1) * (kTileKeys * 128);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           uint32_t v[4];
           e2m1x8_to_h2(cw[i], v);
           const uint32_t sx = i < 2 ? s0 : s1;
-          *reinterpret_cast<uint4*>(block + sw128_offset(key, (unit & 1) * 4 + i)) = make_uint4(h2_mul(v[0], sx), h2_mul(v[1], sx), h2_mul(v[2], sx), h2_mul(v[3], sx));
+          *reinterpret_cast<uint4*>(to + chunk_at[i] + u * (kKeyStep * 128)) = make_uint4(h2_mul(v[0], sx), h2_mul(v[1], sx), h2_mul(v[2], sx), h2_mul(v[3], sx));
         }
       }
     };
@@ -966,39 +990,42 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv4_tile_kernel(AttnArgs a, i
       __syncwarp();
       if (lane == 0) mbar_arrive(bar);
     };
-    auto mark_bad = [&](int t, const int (&pg)[kUnits]) {
-      if (unit != 0) return;
+    auto mark_bad = [&](int t, const uint32_t (&vec)[kUnits]) {
 #pragma unroll
-      for (int u = 0; u < kUnits; ++u) {
-        const int key = key0 + u * kKeyStep, pos = (t0 + t) * kTileKeys + key;
-        if (t < nt && pos < keys && (pg[u] < 1 || pg[u] > a.c.pages)) {
+      for (int u = 0; u < kUnits; ++u)
+        if (vec[u] == kBad && unit == 0) {
+          const int key = key0 + u * kKeyStep;
           dev_fail(a.err, kDevBadPage);
           atomicOr(&bad_keys[t % kTileMarks][key >> 5], 1u << (key & 31));
         }
-      }
     };
     Codes kc, vc;
-    int pg[3][kUnits];  // pages of tiles t, t + 1, t + 2
-    look_up(0, pg[0]);
-    look_up(1, pg[1]);
-    ask(a.c.k, a.c.k_scales, 0, pg[0], kc);
-    mark_bad(0, pg[0]);
+    int page[kUnits];                              // of tile t + 2
+    uint32_t vec[kUnits], vec1[kUnits], vec2[kUnits];  // of tiles t, t + 1, t + 2
+    look_up(0, page);
+    locate(0, page, vec);
+    look_up(1, page);
+    ask(k_unit, ks_unit, vec, kc);
+    mark_bad(0, vec);
+    locate(1, page, vec1);
+    look_up(2, page);
     convert(ks, kc);
     publish(&k_full);
-    ask(a.c.k, a.c.k_scales, 1, pg[1], kc);
+    ask(k_unit, ks_unit, vec1, kc);
     bool ok = true;
     for (int t = 0; t < nt && ok; ++t) {
-      ask(a.c.v, a.c.v_scales, t, pg[0], vc);
-      look_up(t + 2, pg[2]);
+      ask(v_unit, vs_unit, vec, vc);
       if (w < 4) bad_keys[(t + 3) % kTileMarks][w] = 0, nan_keys[(t + 3) % kTileMarks][w] = 0;  // (last used five tiles ago)
       if (t + 1 < nt) {  // K(t + 1), where K(t) was
         ok = wait(&qk_done[t & 1], t >> 1, kDevWaitEmpty);
         if (!ok) break;
-        mark_bad(t + 1, pg[1]);
+        mark_bad(t + 1, vec1);
         convert(ks, kc);
         publish(&k_full);
       }
-      ask(a.c.k, a.c.k_scales, t + 2, pg[2], kc);
+      locate(t + 2, page, vec2);
+      look_up(t + 3, page);
+      ask(k_unit, ks_unit, vec2, kc);
       if ((t0 + t + 1) * kTileKeys > all_see) {  // a masked tile: NaN must not meet the zero probabilities of rows that do not see it
 #pragma unroll
         for (int u = 0; u < kUnits; ++u)
@@ -1013,7 +1040,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv4_tile_kernel(AttnArgs a, i
       convert(vs, vc);
       publish(&v_full);
 #pragma unroll
-      for (int u = 0; u < kUnits; ++u) pg[0][u] = pg[1][u], pg[1][u] = pg[2][u];
+      for (int u = 0; u < kUnits; ++u) vec[u] = vec1[u], vec1[u] = vec2[u];
     }
   } else {
     // ---------------------------------------------------------------- the softmax
@@ -1090,20 +1117,25 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv4_tile_kernel(AttnArgs a, i
         }
       }
       const float base = m == -INFINITY ? 0.f : m - kPShift;
+      uint64_t l2[2] = {0, 0};
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         uint32_t v[32];
         tmem_ld32(s_addr + c * 32, v);
         tmem_ld_wait();
         float p[32];
+        const uint64_t coef2 = f2_pack(coef, coef), base2 = f2_pack(-base, -base);
 #pragma unroll
-        for (int j = 0; j < 32; ++j) p[j] = ex2(fmaf(__uint_as_float(v[j]), coef, -base));
+        for (int j = 0; j < 32; j += 2) {
+          const uint64_t s2 = f2_fma(f2_pack(__uint_as_float(v[j]), __uint_as_float(v[j + 1])), coef2, base2);
+          p[j] = ex2(f2_lo(s2)), p[j + 1] = ex2(f2_hi(s2));
+        }
         if (masked) {
 #pragma unroll
           for (int j = 0; j < 32; ++j) p[j] = vis[c] >> j & 1u ? p[j] : 0.f;
         }
 #pragma unroll
-        for (int j = 0; j < 32; j += 4) l += (p[j] + p[j + 1]) + (p[j + 2] + p[j + 3]);
+        for (int j = 0; j < 32; j += 4) l2[j / 4 & 1] = f2_add(l2[j / 4 & 1], f2_add(f2_pack(p[j], p[j + 1]), f2_pack(p[j + 2], p[j + 3])));
         if (masked) {
           const uint32_t nan = nan_keys[t % kTileMarks][half * 2 + c] & vis[c];
           if (nan) {
@@ -1117,6 +1149,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv4_tile_kernel(AttnArgs a, i
           *reinterpret_cast<uint4*>(to + sw128_offset(r, c * 4 + x)) =
               make_uint4(h2(p[8 * x], p[8 * x + 1]), h2(p[8 * x + 2], p[8 * x + 3]), h2(p[8 * x + 4], p[8 * x + 5]), h2(p[8 * x + 6], p[8 * x + 7]));
       }
+      l += (f2_lo(l2[0]) + f2_hi(l2[0])) + (f2_lo(l2[1]) + f2_hi(l2[1]));
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       tc_fence_before();
       __syncwarp();
