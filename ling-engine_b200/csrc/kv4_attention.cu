@@ -746,18 +746,18 @@ __global__ void __launch_bounds__(kJoinThreads) kv4_join_kernel(AttnArgs a) {
 //                K-major B operand, V, in the same layout, as the value product's MN-major one (no transposition).  K(t+1) comes
 //                before V(t), so that S(t+1) = Q K(t+1)^T runs under the softmax of tile t.  Loads run ahead in registers.
 //   warp 16      one thread issues the MMAs: S(t+1), double in TMEM, then O += P(t) V(t).
-//   warps 0..7   a thread half a row (its TMEM lane, 64 of the tile's keys): maximum, probabilities to FP16 in shared memory, sum; O
-//                is scaled in TMEM only when a score exceeds the row's reference by 2^kLazy.
-// What bounds it is shared memory: operands are read once by the MMAs and written once by the converting warps (D = 256: 224 KB
-// and 160 KB a tile, 3072 cycles at 128 bytes, against 2048 cycles of MMA).
+//   warps 0..7   a thread half a row (its TMEM lane, 64 of the tile's keys): maximum, probabilities to FP16 in TMEM, in the place of
+//                the scores, as the value product's A operand; sum.  O is scaled in TMEM only when a score exceeds the row's
+//                reference by 2^kLazy, so that a tile's softmax need not wait for the tile before.
+// What bounds it is shared memory: operands are read once by the MMAs and written once by the converting warps (D = 256: 192 KB
+// and 128 KB a tile, 2560 cycles at 128 bytes, against 2048 cycles of MMA).
 // Every wait is bounded; one that runs out is recorded and the CTA leaves with its TMEM freed.
 constexpr int kTileRows = 128, kTileKeys = 128, kTileWarps = 17, kTileThreads = kTileWarps * 32, kTileWorkers = 256, kTileMarks = 8;
 constexpr int kMmaWarp = 16;
 template <int D>
 struct TileSmem {
   static constexpr int kOperand = 256 * D;  // 128 rows of D halves: [D / 64][128][128 B]
-  static constexpr int kP = 2 * 128 * 128;  // [2][128 rows][128 B]
-  static constexpr int kBytes = 3 * kOperand + kP + 1024;
+  static constexpr int kBytes = 3 * kOperand + 2 * 2 * kTileRows * 4 + 1024;
 };
 __host__ __device__ constexpr size_t tile_part_floats(int D) { return size_t(kTileRows) * D + 2 * kTileRows; }
 
@@ -765,6 +765,32 @@ __host__ __device__ constexpr size_t tile_part_floats(int D) { return size_t(kTi
 // 1024 bytes apart (stride offset), blocks of 64 mn `lead` bytes (leading offset).
 __device__ __forceinline__ uint64_t desc_mn_sw128(uint32_t addr, uint32_t lead) {
   return uint64_t((addr & 0x3FFFFu) >> 4) | uint64_t(lead >> 4) << 16 | uint64_t(1024 >> 4) << 32 | uint64_t(1) << 46 | uint64_t(2) << 61;
+}
+
+// The eight softmax warps meet: whether all of them are well.
+__device__ __forceinline__ bool meet_all(bool ok) {
+  uint32_t all;
+  asm volatile(
+      "{\n"
+      ".reg .pred p, q;\n"
+      "setp.ne.b32 p, %1, 0;\n"
+      "barrier.red.and.pred q, 1, 256, p;\n"
+      "selp.b32 %0, 1, 0, q;\n"
+      "}\n"
+      : "=r"(all)
+      : "r"(uint32_t(ok))
+      : "memory");
+  return all != 0;
+}
+// D += A B with A in TMEM: lane = row, a column two neighbouring k.
+__device__ __forceinline__ void umma_f16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n"
+      ".reg .pred p;\n"
+      "setp.ne.b32 p, %4, 0;\n"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n"
+      "}\n" ::"r"(tmem_d), "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
 }
 
 template <typename T, int D>
@@ -777,10 +803,10 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv4_tile_kernel(AttnArgs a, i
   uint8_t* qs = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   uint8_t* ks = qs + kOperand;
   uint8_t* vs = ks + kOperand;
-  uint8_t* ps = vs + kOperand;
-  __shared__ uint64_t k_full, v_full, qk_done[2], p_full, pv_done;  // (two score barriers: the next tile's may be done before this one's is waited for)
+  __shared__ uint64_t k_full, v_full, qk_done[2], p_full[2], pv_done[2];  // (by tile parity: a wait knows a phase's parity only, and every one must be waited for in turn)
   __shared__ uint32_t tmem_slot, bad_keys[kTileMarks][4], nan_keys[kTileMarks][4];  // by tile: keys on bad pages; (masked tiles) keys whose V is NaN
-  __shared__ float q_inv[kTileRows], row_max[2][kTileRows];  // (by half; at the end the sums)
+  __shared__ float q_inv[kTileRows];
+  float(*row_max)[2][kTileRows] = reinterpret_cast<float(*)[2][kTileRows]>(vs + kOperand);  // [tile parity][half]; at the end the sums
   __shared__ int where[2];
   __shared__ volatile int failed;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -819,8 +845,10 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv4_tile_kernel(AttnArgs a, i
     mbar_init(&v_full, kTileWorkers / 32);
     mbar_init(&qk_done[0], 1);
     mbar_init(&qk_done[1], 1);
-    mbar_init(&p_full, 8);
-    mbar_init(&pv_done, 1);
+    mbar_init(&p_full[0], 8);
+    mbar_init(&p_full[1], 8);
+    mbar_init(&pv_done[0], 1);
+    mbar_init(&pv_done[1], 1);
     failed = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -919,14 +947,14 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv4_tile_kernel(AttnArgs a, i
       bool ok = scores(0);
       for (int t = 0; t < nt && ok; ++t) {
         if (t + 1 < nt) ok = scores(t + 1);
-        ok = ok && wait(&p_full, t, kDevWaitFull) && wait(&v_full, t, kDevWaitFull);
+        ok = ok && wait(&p_full[t & 1], t >> 1, kDevWaitFull) && wait(&v_full, t, kDevWaitFull);
         if (!ok) break;
         tc_fence_after();
 #pragma unroll
         for (int k = 0; k < kTileKeys / 16; ++k)
-          umma_f16(tmem + kOcol, umma_desc_sw128(smem_u32(ps + (k >> 2) * (kTileRows * 128))) + uint64_t((k & 3) * 2),
-                   desc_mn_sw128(smem_u32(vs + k * 16 * 128), kTileKeys * 128), kIdescO, (t | k) ? 1u : 0u);
-        umma_commit(&pv_done);
+          umma_f16_ts(tmem + kOcol, tmem + uint32_t(t & 1) * kTileKeys + uint32_t((k >> 2) * 64 + (k & 3) * 8),
+                      desc_mn_sw128(smem_u32(vs + k * 16 * 128), kTileKeys * 128), kIdescO, (t | k) ? 1u : 0u);
+        umma_commit(&pv_done[t & 1]);
       }
     }
     __syncwarp();
@@ -1035,7 +1063,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv4_tile_kernel(AttnArgs a, i
             vc.s[u] = 0;
           }
       }
-      ok = wait(&pv_done, t - 1, kDevWaitEmpty);  // V(t), where V(t - 1) was
+      ok = t == 0 || wait(&pv_done[(t - 1) & 1], (t - 1) >> 1, kDevWaitEmpty);  // V(t), where V(t - 1) was
       if (!ok) break;
       convert(vs, vc);
       publish(&v_full);
@@ -1052,9 +1080,10 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv4_tile_kernel(AttnArgs a, i
     const uint32_t lane_addr = tmem + (uint32_t((warp & 3) * 32) << 16);
     float m = -INFINITY, l = 0.f;
     bool ok = true;
-    for (int t = 0; t < nt && ok; ++t) {
-      ok = wait(&qk_done[t & 1], t >> 1, kDevWaitTmemFull);
-      if (ok) tc_fence_after();
+    for (int t = 0; t < nt; ++t) {
+      ok = ok && wait(&qk_done[t & 1], t >> 1, kDevWaitTmemFull);
+      ok = ok && (t < 2 || wait(&pv_done[t & 1], (t - 2) >> 1, kDevWaitTmemFull));  // (done long since: the scores were asked for after it)
+      tc_fence_after();
       const uint32_t s_addr = lane_addr + uint32_t(t & 1) * kTileKeys + half * 64;
       const int base_pos = (t0 + t) * kTileKeys + half * 64;
       uint32_t bad = 0;
@@ -1091,19 +1120,19 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv4_tile_kernel(AttnArgs a, i
           for (int j = 0; j < 32; ++j) mx = fmaxf(mx, __uint_as_float(v[j]));
         }
       }
-      row_max[half][r] = mx;
-      asm volatile("bar.sync 1, 256;" ::: "memory");  // the other half's maximum
-      mx = fmaxf(mx, row_max[half ^ 1][r]);
-      asm volatile("bar.sync 1, 256;" ::: "memory");
-      ok = ok && wait(&pv_done, t - 1, kDevWaitTmemFull);              // P is read, O complete
-      if (masked) ok = ok && wait(&v_full, t, kDevWaitFull);           // the marks of V's NaN
-      tc_fence_after();
+      row_max[t & 1][half][r] = mx;
+      ok = meet_all(ok);  // the other half's maximum; and all eight warps go on, or none
+      if (!ok) break;
+      mx = fmaxf(mx, row_max[t & 1][half ^ 1][r]);
+      if (masked) ok = (t == 0 || wait(&pv_done[(t - 1) & 1], (t - 1) >> 1, kDevWaitTmemFull)) && wait(&v_full, t, kDevWaitFull);  // the marks of V's NaN
       const float top = mx * coef;  // (-inf where nothing is seen)
       const bool grow = top > m + kLazy;
-      if (ok && __any_sync(0xffffffffu, grow)) {
+      if (__any_sync(0xffffffffu, grow)) {
         const float m_new = grow ? top : m, keep = m == -INFINITY ? 0.f : ex2(m - m_new);
         l *= keep, m = m_new;
         if (t > 0) {
+          ok = ok && wait(&pv_done[(t - 1) & 1], (t - 1) >> 1, kDevWaitTmemFull);  // O is complete
+          tc_fence_after();
 #pragma unroll 1
           for (int c = half * (D / 64); c < (half + 1) * (D / 64); ++c) {
             uint32_t x[32];
@@ -1118,6 +1147,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv4_tile_kernel(AttnArgs a, i
       }
       const float base = m == -INFINITY ? 0.f : m - kPShift;
       uint64_t l2[2] = {0, 0};
+      uint32_t pk[32];  // 64 probabilities
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         uint32_t v[32];
@@ -1143,23 +1173,21 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv4_tile_kernel(AttnArgs a, i
             for (int j = 0; j < 32; ++j) p[j] = nan >> j & 1u ? NAN : p[j];
           }
         }
-        uint8_t* to = ps + half * (kTileRows * 128);
 #pragma unroll
-        for (int x = 0; x < 4; ++x)
-          *reinterpret_cast<uint4*>(to + sw128_offset(r, c * 4 + x)) =
-              make_uint4(h2(p[8 * x], p[8 * x + 1]), h2(p[8 * x + 2], p[8 * x + 3]), h2(p[8 * x + 4], p[8 * x + 5]), h2(p[8 * x + 6], p[8 * x + 7]));
+        for (int j = 0; j < 16; ++j) pk[c * 16 + j] = h2(p[2 * j], p[2 * j + 1]);
       }
+      tmem_st32(s_addr, pk);  // where this thread's first 32 scores were: it has read them all
+      tmem_st_wait();
       l += (f2_lo(l2[0]) + f2_hi(l2[0])) + (f2_lo(l2[1]) + f2_hi(l2[1]));
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&p_full);
+      if (lane == 0) mbar_arrive(&p_full[t & 1]);
     }
     // ---- the result, half of the dims a thread
-    row_max[half][r] = l;
-    asm volatile("bar.sync 1, 256;" ::: "memory");
-    l = row_max[0][r] + row_max[1][r];
-    if (ok && wait(&pv_done, nt - 1, kDevWaitTmemFull)) {
+    row_max[nt & 1][half][r] = l;
+    ok = meet_all(ok);
+    l = row_max[nt & 1][0][r] + row_max[nt & 1][1][r];
+    if (ok && wait(&pv_done[(nt - 1) & 1], (nt - 1) >> 1, kDevWaitTmemFull)) {
       tc_fence_after();
       const bool empty = m == -INFINITY && l == 0.f;
       const float scale = empty ? 0.f : a.c.v_scale / l;
