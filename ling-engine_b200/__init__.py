@@ -765,7 +765,7 @@ def describe_tree(parent, chain):
 # ---- a decode layer in 4 bits: operators on DEVICE arrays (anything with data_ptr, shape, stride, dtype and device, as a torch
 # tensor has).  They enqueue on `stream` (a cudaStream_t as an integer; 0 = the default stream) and return.
 F32, BF16, F16 = range(3)
-_ELEMENT = {"torch.float32": F32, "torch.bfloat16": BF16, "torch.float16": F16}
+_ELEMENT = {"torch.float32": F32, "torch.bfloat16": BF16, "torch.float16": F16}  # and, once met, the type objects of these names
 KV4_MAX_SEQS = 1024
 
 
@@ -789,9 +789,19 @@ def _refuse(what):
 
 
 def _device_of(a, what):
-    if not hasattr(a, "data_ptr") or a.device.type != "cuda":
+    if not getattr(a, "is_cuda", False):
         _refuse(what + ": a device array expected")
-    return a.device.index or 0
+    return a.get_device()
+
+
+def _element(dtype, what):
+    t = _ELEMENT.get(dtype)
+    if t is None:
+        t = _ELEMENT.get(str(dtype))
+        if t is None:
+            _refuse(what + ": float32, bfloat16 or float16 expected")
+        _ELEMENT[dtype] = t
+    return t
 
 
 def _words(a, n, what, device, optional=False):
@@ -811,10 +821,10 @@ def _bytes(a, shape, what, device):
 
 def _matrix(a, what, device):
     """(address, element type, row stride) of a device matrix with contiguous rows."""
-    t = _ELEMENT.get(str(a.dtype))
-    if t is None or _device_of(a, what) != device or a.dim() != 2 or (a.shape[1] > 1 and a.stride(1) != 1):
-        _refuse("%s: a matrix of float32, bfloat16 or float16 with contiguous rows on device %d expected" % (what, device))
-    return a.data_ptr(), t, a.stride(0) if a.shape[0] > 1 else max(a.shape[1], 1)
+    shape, stride = a.shape, a.stride()
+    if _device_of(a, what) != device or len(shape) != 2 or (shape[1] > 1 and stride[1] != 1):
+        _refuse("%s: a matrix with contiguous rows on device %d expected" % (what, device))
+    return a.data_ptr(), _element(a.dtype, what), stride[0] if shape[0] > 1 else max(shape[1], 1), shape
 
 
 def _rows_of(a, rows, heads, dim, dtype, what, device):
@@ -834,11 +844,10 @@ def nvfp4_matvec(x, values, scales, alpha, y, accumulate=False, stream=0):
     values [N][K/2], scales [N][K/16] (bytes, as quantize_nvfp4 gives them; alpha carries the tensor scale).  y [M][N] of any of
     the three types.  ling_b200_nvfp4_matvec."""
     device = _device_of(values, "nvfp4_matvec values")
-    xp, xt, ldx = _matrix(x, "nvfp4_matvec x", device)
-    yp, yt, ldy = _matrix(y, "nvfp4_matvec y", device)
-    M, K = x.shape
+    xp, xt, ldx, (M, K) = _matrix(x, "nvfp4_matvec x", device)
+    yp, yt, ldy, y_shape = _matrix(y, "nvfp4_matvec y", device)
     N = values.shape[0]
-    if y.shape[0] != M or y.shape[1] != N or K % 16:
+    if y_shape != (M, N) or K % 16:
         _refuse("nvfp4_matvec: x [M][K], values [N][K/2], y [M][N] with K a multiple of 16 expected")
     fn = lib().ling_b200_nvfp4_matvec
     if fn.argtypes is None:
@@ -893,16 +902,10 @@ class Kv4Cache:
             _refuse(what + ": the batch and the cache are on different devices")
         return None if a is None else _rows_of(a, batch.c.rows, heads, self.head_dim, dtype, what, self.device)
 
-    def _type(self, a, what):
-        t = _ELEMENT.get(str(a.dtype))
-        if t is None:
-            _refuse(what + ": float32, bfloat16 or float16 expected")
-        return t
-
     def append(self, batch, k, v, q=None, q_out=None, rotary_dim=0, theta=1e7, err=None, stream=0):
         """Writes the rows' k, rotated, and v into the cache and rotates q into q_out ([rows][heads][head_dim] each; ling_b200_kv4_append)."""
         heads = 0 if q is None else q.shape[1]
-        check(self._append(self.device, self.ref, batch.ref, self._type(k, "append k"), self._rows(batch, k, self.kv_heads, k.dtype, "append k"),
+        check(self._append(self.device, self.ref, batch.ref, _element(k.dtype, "append k"), self._rows(batch, k, self.kv_heads, k.dtype, "append k"),
                            self._rows(batch, v, self.kv_heads, k.dtype, "append v"), self._rows(batch, q, heads, k.dtype, "append q"), heads,
                            self._rows(batch, q_out, heads, k.dtype, "append q_out"), rotary_dim, theta, _words(err, 1, "append err", self.device, True),
                            stream), "kv4_append")
@@ -912,11 +915,11 @@ class Kv4Cache:
         any_ = k if k is not None else v
         if any_ is None:
             _refuse("read: k or v expected")
-        check(self._read(self.device, self.ref, batch.ref, self._type(any_, "read"), self._rows(batch, k, self.kv_heads, any_.dtype, "read k"),
+        check(self._read(self.device, self.ref, batch.ref, _element(any_.dtype, "read"), self._rows(batch, k, self.kv_heads, any_.dtype, "read k"),
                          self._rows(batch, v, self.kv_heads, any_.dtype, "read v"), _words(err, 1, "read err", self.device, True), stream), "kv4_read")
 
     def attention_workspace_bytes(self, batch, q_heads):
-        """Bytes of the workspace that attention() needs with this batch's bounds (zeroed once by the caller)."""
+        """Bytes of the workspace that attention() needs with this batch's bounds (its contents do not matter)."""
         n = lib().ling_b200_kv4_attention_workspace(self.ref, batch.ref, q_heads)
         if n == 0:
             raise LingError("kv4_attention_workspace failed (status %d): %s" % (ERR_ARG, last_error()))
@@ -931,6 +934,6 @@ class Kv4Cache:
         if lse is not None and (_device_of(lse, "attention lse") != self.device or str(lse.dtype) != "torch.float32" or not lse.is_contiguous() or
                                 lse.numel() < batch.c.rows * heads):
             _refuse("attention: lse [rows][q_heads] of float32 expected")
-        check(self._attention(self.device, self.ref, batch.ref, self._type(q, "attention q"), self._rows(batch, q, heads, q.dtype, "attention q"), heads, scale,
+        check(self._attention(self.device, self.ref, batch.ref, _element(q.dtype, "attention q"), self._rows(batch, q, heads, q.dtype, "attention q"), heads, scale,
                               self._rows(batch, out, heads, q.dtype, "attention out"), None if lse is None else lse.data_ptr(), workspace.data_ptr(),
                               workspace.numel() * workspace.element_size(), _words(err, 1, "attention err", self.device, True), stream), "kv4_attention")

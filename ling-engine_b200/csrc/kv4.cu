@@ -6,6 +6,8 @@
 // found by comparisons alone.  A key's rotation is carried in double and brought to fp32 by rounding to odd (the last bit set
 // when anything was cut off), which keeps every comparison with a value of fewer bits what it is for the exact number: codes
 // do not depend on how fp32 would have rounded the rotation.  Queries need no such care and turn in fp32.
+#include <algorithm>
+
 #include "decode4.cuh"
 
 namespace lb {
@@ -99,38 +101,66 @@ struct AppendArgs {
   int* err;
 };
 
-// A block per packed row; a thread per group of 16 dims of one head's K, V or query vector (the groups of a vector are
+// Where a packed row's vectors go: what a warp finds for the rest of the block.
+struct RowAt {
+  int pos, rope, page;  // page 0: nothing is done for this row
+};
+constexpr int kChunk = kThreads / 32;  // rows of a block at most
+
+// By warp: row r's place.  The error of a row whose sequence or page is out of bounds is recorded here.
+__device__ __forceinline__ RowAt row_at(const ling_b200_kv4& c, const ling_b200_kv4_batch& b, int r, int* err) {
+  RowAt at{0, 0, 0};
+  const int s = kv4_find_seq(b.row0, b.seqs, r);
+  if (s < 0) return at;  // padding behind the last sequence
+  const Kv4Seq q = kv4_seq(c, b, s);
+  at.pos = q.pos + r - q.row0;
+  if (q.ok) {
+    at.page = c.tables[size_t(q.slot) * c.max_pages + at.pos / c.page_tokens];
+    at.rope = b.rope_pos ? b.rope_pos[r] : at.pos;
+  }
+  if (at.page < 1 || at.page > c.pages) {
+    if ((threadIdx.x & 31) == 0) dev_fail(err, q.ok ? int(kDevBadPage) : kDevBadBatch);
+    at.page = 0;
+  }
+  return at;
+}
+
+// A block takes `chunk` packed rows (1 to 8: rows_per_block): a warp per row finds its place, the rows' angles are shared out over
+// the threads, then a thread takes a group of 16 dims of one K, V or query vector at a time (the groups of a vector are
 // neighbouring lanes of one warp).  Floor: the rows read and 9 / 16 byte a value written.
 template <typename T, bool VEC>
-__global__ void __launch_bounds__(kThreads) kv4_append_kernel(AppendArgs a) {
+__global__ void __launch_bounds__(kThreads) kv4_append_kernel(AppendArgs a, int chunk) {
   pdl_sync();  // first statement: see common.cuh
-  __shared__ double2 turn[128];  // cos, sin of the row's angles
-  __shared__ float2 turn32[128];
-  const int r = blockIdx.x, tid = threadIdx.x, lane = tid & 31;
-  const int s = kv4_find_seq(a.b.row0, a.b.seqs, r);
-  if (s < 0) return;  // padding behind the last sequence
-  const Kv4Seq q = kv4_seq(a.c, a.b, s);
-  const int pos = q.pos + r - q.row0, D = a.c.head_dim, groups = D / 16, T_page = a.c.page_tokens;
-  int page = 0;
-  if (q.ok) page = a.c.tables[size_t(q.slot) * a.c.max_pages + pos / T_page];
-  if (!q.ok || page < 1 || page > a.c.pages) {
-    if (tid == 0) dev_fail(a.err, q.ok ? int(kDevBadPage) : kDevBadBatch);
-    return;
+  __shared__ double2 turn[kChunk][128];  // cos, sin of a row's angles
+  __shared__ float2 turn32[kChunk][128];
+  __shared__ double freq[128];
+  __shared__ RowAt rows[kChunk];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, r0 = blockIdx.x * chunk, n = min(chunk, a.b.rows - r0);
+  const int D = a.c.head_dim, groups = D / 16, lg = 31 - __clz(groups), lp = 31 - __clz(a.c.page_tokens), half = a.rot / 2;
+  if (warp < n) {
+    const RowAt at = row_at(a.c, a.b, r0 + warp, a.err);
+    if (lane == 0) rows[warp] = at;
   }
-  const int half = a.rot / 2;
-  const int rp = a.b.rope_pos ? a.b.rope_pos[r] : pos;
-  for (int i = tid; i < half; i += kThreads) {
+  if (tid < half) freq[tid] = pow(a.theta, -2.0 * tid / a.rot);
+  __syncthreads();
+  for (int t = tid; t < n * half; t += kThreads) {
+    const int i = t / half, j = t - i * half;
     double sn, cs;
-    sincos(double(rp) * pow(a.theta, -2.0 * i / a.rot), &sn, &cs);
-    turn[i] = make_double2(cs, sn), turn32[i] = make_float2(float(cs), float(sn));
+    sincos(double(rows[i].rope) * freq[j], &sn, &cs);
+    turn[i][j] = make_double2(cs, sn), turn32[i][j] = make_float2(float(cs), float(sn));
   }
   __syncthreads();
-  const int n_kv = a.c.kv_heads * groups, tasks = 2 * n_kv + a.q_heads * groups;
-  for (int t0 = 0; t0 < tasks; t0 += kThreads) {
-    const int t = t0 + tid;
-    if (t - lane >= tasks) break;  // whole warps: the lanes of a warp exchange below
-    const bool live = t < tasks, is_v = t >= n_kv && t < 2 * n_kv, is_q = t >= 2 * n_kv;
-    const int u = is_q ? t - 2 * n_kv : is_v ? t - n_kv : t, head = u / groups, g = u % groups;
+  const int n_kv = a.c.kv_heads << lg, tasks = 2 * n_kv + (a.q_heads << lg);
+  const double inv64 = 1.0 / double(a.c.k_scale);
+  const float k_inv = 1.f / a.c.k_scale, v_inv = 1.f / a.c.v_scale;  // (powers of two: exact)
+  int i = 0, left = tid;  // task `left` of row i
+  for (; left >= tasks; left -= tasks) ++i;
+  for (int t = tid; t - lane < n * tasks; t += kThreads) {  // whole warps: the lanes of a warp exchange below
+    const int row = i, u_all = left;
+    for (left += kThreads; left >= tasks; left -= tasks) ++i;
+    const bool live = row < n && rows[row].page != 0;
+    const bool is_v = u_all >= n_kv && u_all < 2 * n_kv, is_q = u_all >= 2 * n_kv;
+    const int u = is_q ? u_all - 2 * n_kv : is_v ? u_all - n_kv : u_all, head = u >> lg, g = u & (groups - 1), r = r0 + row;
     const ling_b200_rows& src = is_q ? a.q : is_v ? a.v : a.k;
     const T* vec = static_cast<const T*>(src.p) + r * src.row + head * src.head;
     float x[16] = {};
@@ -150,22 +180,21 @@ __global__ void __launch_bounds__(kThreads) kv4_append_kernel(AppendArgs a) {
             o[j] = d < a.rot ? to_f32<T>(vec[d < half ? d + half : d - half]) : 0.f;
           }
         }
-        const double inv = 1.0 / double(a.c.k_scale);
         double top = 0.0;
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
           const int d = g * 16 + j;
           if (d >= a.rot) {
-            if (!is_q) x[j] *= float(inv), top = fmax(top, fabs(double(x[j]))), bad |= !isfinite(x[j]);
+            if (!is_q) x[j] *= k_inv, top = fmax(top, fabs(double(x[j]))), bad |= !isfinite(x[j]);
             continue;
           }
-          const int i = d < half ? d : d - half;
+          const int at = d < half ? d : d - half;
           if (is_q) {
-            const float2 cs = turn32[i];
+            const float2 cs = turn32[row][at];
             x[j] = d < half ? x[j] * cs.x - o[j] * cs.y : x[j] * cs.x + o[j] * cs.y;
           } else {
-            const double2 cs = turn[i];
-            const double z = (d < half ? double(x[j]) * cs.x - double(o[j]) * cs.y : double(x[j]) * cs.x + double(o[j]) * cs.y) * inv;
+            const double2 cs = turn[row][at];
+            const double z = (d < half ? double(x[j]) * cs.x - double(o[j]) * cs.y : double(x[j]) * cs.x + double(o[j]) * cs.y) * inv64;
             bad |= !(fabs(z) <= 3.402823e38);
             top = fmax(top, fabs(z));
             x[j] = round_to_odd(z);
@@ -173,7 +202,7 @@ __global__ void __launch_bounds__(kThreads) kv4_append_kernel(AppendArgs a) {
         }
         amax6 = float(top / 6.0);
       } else if (!is_q) {
-        const float inv = 1.f / (is_v ? a.c.v_scale : a.c.k_scale);
+        const float inv = is_v ? v_inv : k_inv;
         float top = 0.f;
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
@@ -185,13 +214,13 @@ __global__ void __launch_bounds__(kThreads) kv4_append_kernel(AppendArgs a) {
       }
     }
     // a vector with a value that is not finite is NaN whole; the ballot also keeps a query's stores behind all loads of its vector
-    const unsigned any = __ballot_sync(0xffffffffu, bad) >> (lane / groups * groups) & ((1u << groups) - 1u);
+    const unsigned any = __ballot_sync(0xffffffffu, bad) >> (lane >> lg << lg) & ((1u << groups) - 1u);
     if (!live) continue;
     if (is_q) {
       store16<T, VEC>(static_cast<T*>(a.q_out.p) + r * a.q_out.row + head * a.q_out.head + g * 16, x);
       continue;
     }
-    const size_t at = kv4_vector(a.c, page, head, pos % T_page);
+    const size_t at = kv4_vector(a.c, rows[row].page, head, rows[row].pos & ((1 << lp) - 1));
     uint8_t code = to_e4m3(fminf(fmaxf(amax6, 0x1p-9f), 448.f));
     const float sc = from_e4m3(code);
     uint2 w = make_uint2(e2m1_codes(x, sc), e2m1_codes(x + 8, sc));
@@ -208,45 +237,53 @@ struct ReadArgs {
   int* err;
 };
 
+// As the append, the other way: a thread per group of 16 dims, read, decoded and stored.
 template <typename T, bool VEC>
-__global__ void __launch_bounds__(kThreads) kv4_read_kernel(ReadArgs a) {
+__global__ void __launch_bounds__(kThreads) kv4_read_kernel(ReadArgs a, int chunk) {
   pdl_sync();  // first statement: see common.cuh
-  const int r = blockIdx.x;
-  const int s = kv4_find_seq(a.b.row0, a.b.seqs, r);
-  if (s < 0) return;
-  const Kv4Seq q = kv4_seq(a.c, a.b, s);
-  const int pos = q.pos + r - q.row0, D = a.c.head_dim, groups = D / 16, T_page = a.c.page_tokens, n_kv = a.c.kv_heads * groups;
-  int page = 0;
-  if (q.ok) page = a.c.tables[size_t(q.slot) * a.c.max_pages + pos / T_page];
-  if (!q.ok || page < 1 || page > a.c.pages) {
-    if (threadIdx.x == 0) dev_fail(a.err, q.ok ? int(kDevBadPage) : kDevBadBatch);
-    return;
+  __shared__ RowAt rows[kChunk];
+  const int tid = threadIdx.x, warp = tid >> 5, r0 = blockIdx.x * chunk, n = min(chunk, a.b.rows - r0);
+  const int D = a.c.head_dim, groups = D / 16, lg = 31 - __clz(groups), lp = 31 - __clz(a.c.page_tokens), n_kv = a.c.kv_heads << lg;
+  if (warp < n) {
+    const RowAt at = row_at(a.c, a.b, r0 + warp, a.err);
+    if ((tid & 31) == 0) rows[warp] = at;
   }
-  for (int t = threadIdx.x; t < 2 * n_kv; t += kThreads) {
-    const bool is_v = t >= n_kv;
-    const int u = is_v ? t - n_kv : t, head = u / groups, g = u % groups;
+  __syncthreads();
+  int i = 0, left = tid;
+  for (; left >= 2 * n_kv; left -= 2 * n_kv) ++i;
+  while (i < n) {
+    const int row = i, u_all = left;
+    for (left += kThreads; left >= 2 * n_kv; left -= 2 * n_kv) ++i;
+    const bool is_v = u_all >= n_kv;
+    const int u = is_v ? u_all - n_kv : u_all, head = u >> lg, g = u & (groups - 1);
     const ling_b200_rows& to = is_v ? a.v : a.k;
-    if (!to.p) continue;
-    const size_t at = kv4_vector(a.c, page, head, pos % T_page);
+    if (!to.p || rows[row].page == 0) continue;
+    const size_t at = kv4_vector(a.c, rows[row].page, head, rows[row].pos & ((1 << lp) - 1));
     float x[16];
     decode16(reinterpret_cast<const uint2*>((is_v ? a.c.v : a.c.k) + at * (D / 2))[g],
              from_e4m3((is_v ? a.c.v_scales : a.c.k_scales)[at * groups + g]) * (is_v ? a.c.v_scale : a.c.k_scale), x);
-    store16<T, VEC>(static_cast<T*>(to.p) + r * to.row + head * to.head + g * 16, x);
+    store16<T, VEC>(static_cast<T*>(to.p) + (r0 + row) * to.row + head * to.head + g * 16, x);
   }
 }
+
+// Rows of a block: one while the SMs are not filled (a row's chain of lookups is what a small batch takes), eight when they are
+// filled many times over (the frequencies and the lookups' latency are then shared by eight rows).
+inline int rows_per_block(int rows, int sms) { return std::min(kChunk, std::max(1, rows / (4 * sms))); }
 
 DeviceInfo g_devices[kMaxDevices];
 std::mutex g_mutex;
 
 template <typename T>
-int append_launch(const AppendArgs& a, bool vec, cudaStream_t s) {
-  LB_CUDA(launch_kernel(vec ? kv4_append_kernel<T, true> : kv4_append_kernel<T, false>, dim3(a.b.rows), dim3(kThreads), size_t(0), s, a));
+int append_launch(const AppendArgs& a, bool vec, int sms, cudaStream_t s) {
+  const int chunk = rows_per_block(a.b.rows, sms);
+  LB_CUDA(launch_kernel(vec ? kv4_append_kernel<T, true> : kv4_append_kernel<T, false>, dim3((a.b.rows + chunk - 1) / chunk), dim3(kThreads), size_t(0), s, a, chunk));
   LB_LAUNCH("kv4_append_kernel");
   return LING_B200_OK;
 }
 template <typename T>
-int read_launch(const ReadArgs& a, bool vec, cudaStream_t s) {
-  LB_CUDA(launch_kernel(vec ? kv4_read_kernel<T, true> : kv4_read_kernel<T, false>, dim3(a.b.rows), dim3(kThreads), size_t(0), s, a));
+int read_launch(const ReadArgs& a, bool vec, int sms, cudaStream_t s) {
+  const int chunk = rows_per_block(a.b.rows, sms);
+  LB_CUDA(launch_kernel(vec ? kv4_read_kernel<T, true> : kv4_read_kernel<T, false>, dim3((a.b.rows + chunk - 1) / chunk), dim3(kThreads), size_t(0), s, a, chunk));
   LB_LAUNCH("kv4_read_kernel");
   return LING_B200_OK;
 }
@@ -284,7 +321,7 @@ extern "C" int ling_b200_kv4_append(int device, const ling_b200_kv4* cache, cons
   bool vec = rows_vec(*k, type) && rows_vec(*v, type) && (rotary_dim / 2 % 16 != 0 || rotary_dim / 2 * type_size(type) % 16 == 0);
   if (q) a.q = *q, a.q_out = *q_out, a.q_heads = q_heads, vec = vec && rows_vec(*q, type) && rows_vec(*q_out, type);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  return type == LING_B200_F32 ? append_launch<float>(a, vec, s) : type == LING_B200_BF16 ? append_launch<__nv_bfloat16>(a, vec, s) : append_launch<__half>(a, vec, s);
+  return type == LING_B200_F32 ? append_launch<float>(a, vec, sms, s) : type == LING_B200_BF16 ? append_launch<__nv_bfloat16>(a, vec, sms, s) : append_launch<__half>(a, vec, sms, s);
 }
 
 extern "C" int ling_b200_kv4_read(int device, const ling_b200_kv4* cache, const ling_b200_kv4_batch* batch, int type, const ling_b200_rows* k,
@@ -305,5 +342,5 @@ extern "C" int ling_b200_kv4_read(int device, const ling_b200_kv4* cache, const 
   const ReadArgs a{*cache, *batch, k ? *k : ling_b200_rows{nullptr, 0, 0}, v ? *v : ling_b200_rows{nullptr, 0, 0}, err};
   const bool vec = (!k || rows_vec(*k, type)) && (!v || rows_vec(*v, type));
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  return type == LING_B200_F32 ? read_launch<float>(a, vec, s) : type == LING_B200_BF16 ? read_launch<__nv_bfloat16>(a, vec, s) : read_launch<__half>(a, vec, s);
+  return type == LING_B200_F32 ? read_launch<float>(a, vec, sms, s) : type == LING_B200_BF16 ? read_launch<__nv_bfloat16>(a, vec, sms, s) : read_launch<__half>(a, vec, sms, s);
 }
