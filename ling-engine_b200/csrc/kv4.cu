@@ -7,6 +7,7 @@
 // when anything was cut off), which keeps every comparison with a value of fewer bits what it is for the exact number: codes
 // do not depend on how fp32 would have rounded the rotation.  Queries need no such care and turn in fp32.
 #include <algorithm>
+#include <cfloat>
 
 #include "decode4.cuh"
 
@@ -125,9 +126,19 @@ __device__ __forceinline__ RowAt row_at(const ling_b200_kv4& c, const ling_b200_
   return at;
 }
 
+// u / per and the rest for u < 2^18 and per <= 256, without a division (u times the reciprocal's error stays below 2^32).
+struct Split {
+  int per;
+  uint32_t inv;
+  __device__ explicit Split(int p) : per(p), inv(p > 1 ? 0xffffffffu / uint32_t(p) + 1u : 0u) {}
+  __device__ int head(int u) const { return per > 1 ? int(__umulhi(uint32_t(u), inv)) : u; }
+};
+
 // A block takes `chunk` packed rows (1 to 8: rows_per_block): a warp per row finds its place, the rows' angles are shared out over
-// the threads, then a thread takes a group of 16 dims of one K, V or query vector at a time (the groups of a vector are
-// neighbouring lanes of one warp).  Floor: the rows read and 9 / 16 byte a value written.
+// the threads, then a thread takes a group of 16 dims of one K or V vector at a time (the groups of a vector are neighbouring lanes
+// of one warp), then 16 pairs of dims of a query that turn together, then 16 bytes of the queries' dims that do not turn.  What a
+// warp executes is of one kind: a query's turning dims beside its resting ones, lane by lane, cost three times the instructions.
+// Floor: the rows read and 9 / 16 byte a value written.
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(kThreads) kv4_append_kernel(AppendArgs a, int chunk) {
   pdl_sync();  // first statement: see common.cuh
@@ -150,18 +161,16 @@ __global__ void __launch_bounds__(kThreads) kv4_append_kernel(AppendArgs a, int 
     turn[i][j] = make_double2(cs, sn), turn32[i][j] = make_float2(float(cs), float(sn));
   }
   __syncthreads();
-  const int n_kv = a.c.kv_heads << lg, tasks = 2 * n_kv + (a.q_heads << lg);
+  const int n_kv = a.c.kv_heads << lg;
   const double inv64 = 1.0 / double(a.c.k_scale);
   const float k_inv = 1.f / a.c.k_scale, v_inv = 1.f / a.c.v_scale;  // (powers of two: exact)
-  int i = 0, left = tid;  // task `left` of row i
-  for (; left >= tasks; left -= tasks) ++i;
-  for (int t = tid; t - lane < n * tasks; t += kThreads) {  // whole warps: the lanes of a warp exchange below
-    const int row = i, u_all = left;
-    for (left += kThreads; left >= tasks; left -= tasks) ++i;
-    const bool live = row < n && rows[row].page != 0;
-    const bool is_v = u_all >= n_kv && u_all < 2 * n_kv, is_q = u_all >= 2 * n_kv;
-    const int u = is_q ? u_all - 2 * n_kv : is_v ? u_all - n_kv : u_all, head = u >> lg, g = u & (groups - 1), r = r0 + row;
-    const ling_b200_rows& src = is_q ? a.q : is_v ? a.v : a.k;
+  const bool whole = half % 16 == 0;  // a group's dims turn all in one way or not at all
+  // ---- K and V into the cache
+  for (int t = tid; t - lane < n * 2 * n_kv; t += kThreads) {  // whole warps: the lanes of a warp exchange below
+    const int row = t / (2 * n_kv), u_all = t - row * (2 * n_kv);
+    const bool live = row < n && rows[row].page != 0, is_v = u_all >= n_kv;
+    const int u = is_v ? u_all - n_kv : u_all, head = u >> lg, g = u & (groups - 1), r = r0 + row;
+    const ling_b200_rows& src = is_v ? a.v : a.k;
     const T* vec = static_cast<const T*>(src.p) + r * src.row + head * src.head;
     float x[16] = {};
     bool bad = false;
@@ -169,39 +178,39 @@ __global__ void __launch_bounds__(kThreads) kv4_append_kernel(AppendArgs a, int 
     if (live) {
       load16<T, VEC>(vec + g * 16, x);
       if (!is_v && g * 16 < a.rot) {
-        float o[16];  // the dims these turn with
-        const bool whole = half % 16 == 0;
+        double top = 0.0;
+        auto turned = [&](int j, double z) {
+          bad |= !(fabs(z) <= double(FLT_MAX));
+          top = fmax(top, fabs(z));
+          x[j] = round_to_odd(z);
+        };
         if (whole) {
-          load16<T, VEC>(vec + (g * 16 < half ? g * 16 + half : g * 16 - half), o);
+          const bool low = g * 16 < half;
+          const int at = low ? g * 16 : g * 16 - half;
+          float o[16];  // the dims these turn with
+          load16<T, VEC>(vec + (low ? g * 16 + half : at), o);
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            const double2 cs = turn[row][at + j];
+            const double sn = low ? -cs.y : cs.y;
+            turned(j, (double(x[j]) * cs.x + double(o[j]) * sn) * inv64);
+          }
         } else {
 #pragma unroll
           for (int j = 0; j < 16; ++j) {
             const int d = g * 16 + j;
-            o[j] = d < a.rot ? to_f32<T>(vec[d < half ? d + half : d - half]) : 0.f;
-          }
-        }
-        double top = 0.0;
-#pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          const int d = g * 16 + j;
-          if (d >= a.rot) {
-            if (!is_q) x[j] *= k_inv, top = fmax(top, fabs(double(x[j]))), bad |= !isfinite(x[j]);
-            continue;
-          }
-          const int at = d < half ? d : d - half;
-          if (is_q) {
-            const float2 cs = turn32[row][at];
-            x[j] = d < half ? x[j] * cs.x - o[j] * cs.y : x[j] * cs.x + o[j] * cs.y;
-          } else {
-            const double2 cs = turn[row][at];
-            const double z = (d < half ? double(x[j]) * cs.x - double(o[j]) * cs.y : double(x[j]) * cs.x + double(o[j]) * cs.y) * inv64;
-            bad |= !(fabs(z) <= 3.402823e38);
-            top = fmax(top, fabs(z));
-            x[j] = round_to_odd(z);
+            if (d >= a.rot) {
+              turned(j, double(x[j]) * inv64);
+              continue;
+            }
+            const bool low = d < half;
+            const double2 cs = turn[row][low ? d : d - half];
+            const double o = double(to_f32<T>(vec[low ? d + half : d - half]));
+            turned(j, (double(x[j]) * cs.x + o * (low ? -cs.y : cs.y)) * inv64);
           }
         }
         amax6 = float(top / 6.0);
-      } else if (!is_q) {
+      } else {
         const float inv = is_v ? v_inv : k_inv;
         float top = 0.f;
 #pragma unroll
@@ -213,13 +222,9 @@ __global__ void __launch_bounds__(kThreads) kv4_append_kernel(AppendArgs a, int 
         amax6 = __fdiv_rn(top, 6.f);
       }
     }
-    // a vector with a value that is not finite is NaN whole; the ballot also keeps a query's stores behind all loads of its vector
+    // a vector with a value that is not finite is NaN whole
     const unsigned any = __ballot_sync(0xffffffffu, bad) >> (lane >> lg << lg) & ((1u << groups) - 1u);
     if (!live) continue;
-    if (is_q) {
-      store16<T, VEC>(static_cast<T*>(a.q_out.p) + r * a.q_out.row + head * a.q_out.head + g * 16, x);
-      continue;
-    }
     const size_t at = kv4_vector(a.c, rows[row].page, head, rows[row].pos & ((1 << lp) - 1));
     uint8_t code = to_e4m3(fminf(fmaxf(amax6, 0x1p-9f), 448.f));
     const float sc = from_e4m3(code);
@@ -227,6 +232,65 @@ __global__ void __launch_bounds__(kThreads) kv4_append_kernel(AppendArgs a, int 
     if (any) w = make_uint2(0, 0), code = 0x7f;
     reinterpret_cast<uint2*>((is_v ? a.c.v : a.c.k) + at * (D / 2))[g] = w;
     (is_v ? a.c.v_scales : a.c.k_scales)[at * groups + g] = code;
+  }
+  if (a.q_heads == 0) return;
+  // ---- the queries' turning dims: a thread has both dims of its pairs, so q_out may be q
+  const T* q = static_cast<const T*>(a.q.p);
+  T* q_out = static_cast<T*>(a.q_out.p);
+  const Split pairs((half + 15) / 16);
+  for (int t = tid, per = a.q_heads * pairs.per; t < n * per; t += kThreads) {
+    const int row = t / per, u = t - row * per, head = pairs.head(u), i0 = (u - head * pairs.per) * 16;
+    if (rows[row].page == 0) continue;
+    const T* from = q + (r0 + row) * a.q.row + head * a.q.head + i0;
+    T* to = q_out + (r0 + row) * a.q_out.row + head * a.q_out.head + i0;
+    if (whole) {
+      float x[16], o[16];
+      load16<T, VEC>(from, x);
+      load16<T, VEC>(from + half, o);
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        const float2 cs = turn32[row][i0 + j];
+        const float y = x[j] * cs.x - o[j] * cs.y;
+        o[j] = x[j] * cs.y + o[j] * cs.x, x[j] = y;
+      }
+      store16<T, VEC>(to, x);
+      store16<T, VEC>(to + half, o);
+    } else {
+      for (int j = 0; j < 16 && i0 + j < half; ++j) {
+        const float2 cs = turn32[row][i0 + j];
+        const float x = to_f32<T>(from[j]), o = to_f32<T>(from[j + half]);
+        to[j] = from_f32<T>(x * cs.x - o * cs.y), to[j + half] = from_f32<T>(x * cs.y + o * cs.x);
+      }
+    }
+  }
+  // ---- and those that do not turn, where q_out is not q
+  if (a.rot == D || (a.q.p == a.q_out.p && a.q.row == a.q_out.row && a.q.head == a.q_out.head)) return;
+  if (VEC && whole) {
+    constexpr int kPer = 16 / sizeof(T), kFly = 4;
+    const Split pieces((D - a.rot) / kPer);
+    const int per = a.q_heads * pieces.per;
+    for (int t0 = tid; t0 < n * per; t0 += kThreads * kFly) {
+      uint4 w[kFly];
+      T* to[kFly];
+#pragma unroll
+      for (int f = 0; f < kFly; ++f) {
+        const int t = t0 + f * kThreads, row = t / per, u = t - row * per, head = pieces.head(u), d = a.rot + (u - head * pieces.per) * kPer;
+        to[f] = nullptr;
+        if (t < n * per && rows[row].page != 0) {
+          w[f] = *reinterpret_cast<const uint4*>(q + (r0 + row) * a.q.row + head * a.q.head + d);
+          to[f] = q_out + (r0 + row) * a.q_out.row + head * a.q_out.head + d;
+        }
+      }
+#pragma unroll
+      for (int f = 0; f < kFly; ++f)
+        if (to[f]) *reinterpret_cast<uint4*>(to[f]) = w[f];
+    }
+  } else {
+    const Split rest(D - a.rot);
+    for (int t = tid, per = a.q_heads * rest.per; t < n * per; t += kThreads) {
+      const int row = t / per, u = t - row * per, head = rest.head(u), d = a.rot + u - head * rest.per;
+      if (rows[row].page != 0) q_out[(r0 + row) * a.q_out.row + head * a.q_out.head + d] = q[(r0 + row) * a.q.row + head * a.q.head + d];
+    }
   }
 }
 
