@@ -713,7 +713,7 @@ typedef struct ling_b200_kv4 {
   float k_scale, v_scale;
 } ling_b200_kv4;
 /* The packed rows of a call: rows row0[s] .. row0[s+1] are sequence s, its row i stands at position pos[s] + i of the slot's table
- * (ragged, a sequence may have none; rows from row0[seqs] on are padding and are left as they were).  Device arrays; the bounds
+ * (ragged, a sequence may have none; rows from row0[seqs] on are padding and are left as they were).  row0 does not descend.  Device arrays; the bounds
  * are the host's: a sequence outside them is skipped and recorded in err. */
 typedef struct ling_b200_kv4_batch {
   const int *row0, *slot, *pos; /* [seqs + 1], [seqs], [seqs] */
@@ -730,7 +730,7 @@ typedef struct ling_b200_rows {
 } ling_b200_rows;
 
 /* Writes the rows' K, rotated, and V, as they are, into the cache, and rotates the rows' queries beside them (q and q_out with q_heads
- * heads, or both NULL; q_out may be q).  The rotation is attn_prepare's: dims d and d + rotary_dim / 2 of the first rotary_dim
+ * heads, or both NULL; q_out may be q, or must not overlap it, k or v).  The rotation is attn_prepare's: dims d and d + rotary_dim / 2 of the first rotary_dim
  * dims (even, 0 = none) turn by rope_pos * theta^(-2 d / rotary_dim).  Per 16 dims the scale is E4M3(clamp(amax / 6, 2^-9, 448)) and
  * a code the nearest, a value halfway between two the smaller magnitude (ling_b200_quantize_nvfp4_host's rule); the rotation
  * of keys and every comparison are carried beyond fp32, so codes are those of the exact values.  A K or V vector with a value that is not
@@ -747,8 +747,8 @@ int ling_b200_kv4_read(int device, const ling_b200_kv4* cache, const ling_b200_k
  * already rotated; out has its type.  lse [rows][q_heads], or NULL: log of the sum of exp(scale * q . k).  A row that sees nothing
  * has out 0 and lse -inf; NaN or infinities at positions a row does not see do not reach it.  `workspace` holds the partial
  * results of contexts that are split over SMs: as many bytes as ling_b200_kv4_attention_workspace says for the same cache
- * dims, batch bounds and q_heads, 16-byte aligned, zeroed once before its first use and then left alone; calls that may overlap
- * on the GPU (other streams, graphs launched together) need one each. */
+ * dims, batch bounds and q_heads, 16-byte aligned; what it holds before a call does not matter, and calls that may overlap on
+ * the GPU (other streams, graphs launched together) need one each. */
 size_t ling_b200_kv4_attention_workspace(const ling_b200_kv4* cache, const ling_b200_kv4_batch* batch, int q_heads);
 int ling_b200_kv4_attention(int device, const ling_b200_kv4* cache, const ling_b200_kv4_batch* batch, int type, const ling_b200_rows* q,
                             int q_heads, float scale, const ling_b200_rows* out, float* lse, void* workspace, size_t workspace_bytes,

@@ -71,12 +71,6 @@ __device__ __forceinline__ void store16(T* p, const float (&x)[16]) {
 }
 
 // ---------------------------------------------------------------------------------------------- NVFP4
-// Magnitude and sign of one E2M1 code: s eem, 0 0.5 1 1.5 2 3 4 6.
-__device__ __forceinline__ float from_e2m1(uint32_t c) {
-  const uint32_t e = (c >> 1) & 3u, m = c & 1u;
-  const float v = e == 0 ? 0.5f * float(m) : (1.f + 0.5f * float(m)) * float(1u << (e - 1));
-  return c & 8u ? -v : v;
-}
 // Two codes of a byte (the first in the low nibble) as two halves, exactly.
 __device__ __forceinline__ uint32_t e2m1x2_to_h2(uint32_t byte) {
   uint32_t r;

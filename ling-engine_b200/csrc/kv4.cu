@@ -28,6 +28,8 @@ bool kv4_cache_ok(const ling_b200_kv4* c, const char* who) {
   if (c->kv_heads < 1 || c->kv_heads > 1024 || c->pages < 1 || c->slots < 1 || c->max_pages < 1 ||
       c->max_pages > (1 << 30) / c->page_tokens)
     return no("a cache size out of range");
+  if ((long long)c->pages >= (1ll << 32) / ((long long)c->kv_heads * c->page_tokens) - 1)  // (the kernels' vector indices have 32 bits)
+    return no("the cache holds 2^32 vectors or more");
   for (float s : {c->k_scale, c->v_scale}) {
     int e = 0;
     if (!(s >= 0x1p-30f && s <= 0x1p30f) || std::frexp(s, &e) != 0.5f) return no("k_scale and v_scale must be powers of two in [2^-30, 2^30]");

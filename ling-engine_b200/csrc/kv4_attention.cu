@@ -161,6 +161,8 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// What a row's raw scores are worth as powers of two; never 0 (a scale of 0, or a product below fp32): a masked score is -inf.
+__device__ __forceinline__ float score_coef(const AttnArgs& a, float q_inv) { return fmaxf(fabsf(a.scale) * a.c.k_scale * kLog2e * q_inv, 0x1p-126f); }
 // What a partial result (reference m, sum l) counts for under the common reference: one without a visible key has l = 0, one whose
 // scores were all NaN has l = NaN and no m.
 __device__ __forceinline__ float part_weight(float m, float l, float common) { return m == -INFINITY ? (l == 0.f ? 0.f : 1.f) : ex2(m - common); }
@@ -415,7 +417,7 @@ __global__ void __launch_bounds__(kDecThreads, 1) kv4_decode_kernel(AttnArgs a) 
     uint32_t see[2];  // in-flight rows each sees, as a mask or (no masks) their number
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-      coef[j] = fabsf(a.scale) * a.c.k_scale * kLog2e * __shfl_sync(0xffffffffu, inv, (2 * t + j) * 4);
+      coef[j] = score_coef(a, __shfl_sync(0xffffffffu, inv, (2 * t + j) * 4));
       const int i = (tile * kDecRows + 2 * t + j) / G;
       see[j] = i >= sq.n ? 0u : a.b.anc ? a.b.anc[sq.row0 + i] : uint32_t(i + 1);
     }
@@ -1074,7 +1076,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv4_tile_kernel(AttnArgs a, i
     // ---------------------------------------------------------------- the softmax
     const int r = tid & (kTileRows - 1), half = tid >> 7, f = f0 + r, i_row = f / G;  // row r, keys half * 64 .. + 64 of a tile
     const bool real = f < R;
-    const float coef = fabsf(a.scale) * a.c.k_scale * kLog2e * q_inv[r];
+    const float coef = score_coef(a, q_inv[r]);
     const uint32_t see = real && a.b.anc ? a.b.anc[sq.row0 + i_row] : 0u;
     const int limit = real ? sq.pos + i_row + 1 : 0;  // (no masks) positions this row sees
     const uint32_t lane_addr = tmem + (uint32_t((warp & 3) * 32) << 16);
@@ -1231,7 +1233,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv4_tile_kernel(AttnArgs a, i
 
 // The splits' partial results of the tile kernel: a warp a query row, in the order of the splits.
 template <typename T, int D>
-__global__ void __launch_bounds__(256) kv4_tile_join_kernel(AttnArgs a, int splits) {
+__global__ void __launch_bounds__(256) kv4_tile_join_kernel(AttnArgs a, int splits, int row_tiles) {
   pdl_sync();  // first statement: see common.cuh
   const int lane = threadIdx.x & 31, G = a.q_heads / a.c.kv_heads, H = a.c.kv_heads, h = blockIdx.y;
   const int r = blockIdx.x * 8 + (threadIdx.x >> 5);  // packed row * G + head of the group
@@ -1260,6 +1262,7 @@ __global__ void __launch_bounds__(256) kv4_tile_join_kernel(AttnArgs a, int spli
   }
   if (seq < 0) return;
   const int f = (row - a.b.row0[seq]) * G + r % G, in = f % kTileRows;
+  if (tile0 + f / kTileRows >= row_tiles) return;  // (sequences that share rows, against the batch's rules: more tiles than rows have)
   const float* parts = a.parts + (size_t(tile0 + f / kTileRows) * H + h) * splits * tile_part_floats(D);
   float mm = -INFINITY;
   for (int s = 0; s < splits; ++s) mm = fmaxf(mm, parts[s * tile_part_floats(D) + kTileRows * D + in]);
@@ -1346,7 +1349,7 @@ int tile_launch_t(const AttnArgs& a, const Plan& p, cudaStream_t s) {
   LB_CUDA(launch_kernel(kv4_tile_kernel<T, D>, dim3(p.row_tiles, a.c.kv_heads, p.splits), dim3(kTileThreads), size_t(TileSmem<D>::kBytes), s, a, p.splits));
   LB_LAUNCH("kv4_tile_kernel");
   if (p.splits > 1) {
-    LB_CUDA(launch_dependent(kv4_tile_join_kernel<T, D>, dim3(ceil_div(a.b.rows * (a.q_heads / a.c.kv_heads), 8), a.c.kv_heads), dim3(256), size_t(0), s, a, p.splits));
+    LB_CUDA(launch_dependent(kv4_tile_join_kernel<T, D>, dim3(ceil_div(a.b.rows * (a.q_heads / a.c.kv_heads), 8), a.c.kv_heads), dim3(256), size_t(0), s, a, p.splits, p.row_tiles));
     LB_LAUNCH("kv4_tile_join_kernel");
   }
   return LING_B200_OK;

@@ -119,7 +119,7 @@ def calls(lb, cache, batch, rows=(4096, 256, 128), type_=1, q_heads=4, rot=64, t
 
 @pytest.mark.parametrize("change", [dict(k=0), dict(tables=0), dict(k=4100), dict(v_scales=32770), dict(head_dim=96), dict(page_tokens=48), dict(page_tokens=8),
                                     dict(kv_heads=0), dict(pages=0), dict(slots=0), dict(max_pages=0), dict(k_scale=0.3), dict(v_scale=0.0), dict(k_scale=math.nan),
-                                    dict(v_scale=2.0 ** 31)])
+                                    dict(v_scale=2.0 ** 31), dict(pages=1 << 27), dict(pages=(1 << 31) - 1)])
 def test_cache_refusals(lb, change):
     assert calls(lb, c_cache(lb, **change), c_batch(lb)) == (lb.ERR_ARG,) * 3 and lb.last_error()
 
@@ -354,6 +354,15 @@ def test_append(gpu, lb, D, H, q_heads, rot, page, layout, t):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("D,H,q_heads,rot,layout,t", [(64, 2, 3, 32, "slice", "bf16"), (64, 2, 3, 36, "apart", "f32"), (128, 1, 5, 20, "slice", "f16"), (256, 1, 2, 256, "odd", "bf16"),
+                                                      (128, 1, 1, 0, "apart", "bf16")])
+def test_append_many_rows(gpu, lb, D, H, q_heads, rot, layout, t):
+    """Several rows a block: blocks that cross from one sequence to the next, and into the padding."""
+    s = Setup(lb, [(1201, 5), (0, 3), (2500, 700), (1, 77), (6, 0), (1003, 16)], D, H, 16, seed=rot, fill=0x33, padded=13)
+    check_append(lb, s, t, q_heads, rot, layout=layout)
+
+
+@pytest.mark.gpu
 def test_append_one_token_many_sequences_far_positions(gpu, lb):
     s = Setup(lb, [(1, 37 * i) for i in range(70)] + [(1, 131071)], 128, 2, 64, seed=3, fill=0)
     rope = torch.randint(0, 1 << 24, (s.rows,), device="cuda", generator=s.gen).int()
@@ -416,7 +425,7 @@ def test_append_and_read_skip_and_record_what_is_out_of_bounds(gpu, lb):
 def check_attention(lb, s, t, G, scale=None, spread=1.0, layout="apart", k_scale=1.0, v_scale=1.0, lse=True, q=None, err_code=0, work=None, skip=None):
     D, H, R = s.D, s.H, s.rows
     Q = H * G
-    scale = scale or 1 / math.sqrt(D)
+    scale = 1 / math.sqrt(D) if scale is None else scale
     if q is None:
         q = torch.randn(R, Q, D, device="cuda", generator=s.gen) * spread
     if layout == "slice":
@@ -454,7 +463,7 @@ def check_attention(lb, s, t, G, scale=None, spread=1.0, layout="apart", k_scale
             o = torch.where(see.any(-1, keepdim=True), o, 0.0)
             A = (e @ vh.abs().nan_to_num(0)) / l.clamp(min=1e-300)
             tail = (see.double() @ vh.abs().nan_to_num(0)) / l.clamp(min=1.0)
-            E = 2.0 ** -23 * (D + 8) * scale * (qh.abs() @ kh.abs().nan_to_num(0).t()).amax(-1, keepdim=True)
+            E = 2.0 ** -23 * (D + 8) * abs(scale) * (qh.abs() @ kh.abs().nan_to_num(0).t()).amax(-1, keepdim=True)
             tol = torch.finfo(T[t]).eps / 2 * o.abs() + (2.0 ** -11 + 2 * E + 2.0 ** -19) * A + 2.0 ** -33 * tail + 2.0 ** -24 * (t == "f16")
             got = out[a:a + r, h].double()
             assert torch.equal(torch.isnan(got), torch.isnan(o)), (i, h)
@@ -555,6 +564,52 @@ def test_attention_long_context_and_bounds_looser_than_the_lengths(gpu, lb):
     b.max_context, b.max_rows = 60000, 4
     b.rows = b.total
     check_attention(lb, b, "bf16", 6)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [1, 3, 40])
+def test_attention_scales_below_zero_and_none(gpu, lb, rows):
+    s = Setup(lb, [(rows, 90), (rows, 0), (rows, 700)], 64, 2, 16, seed=15 + rows)
+    check_attention(lb, s, "bf16", 3, scale=-0.2)
+    check_attention(lb, s, "bf16", 3, scale=0.0)                                                        # a plain mean of what a row sees
+    check_attention(lb, s, "bf16", 3, scale=1e-30, q=torch.full((s.rows, 6, 64), 1e-30, device="cuda"))  # a product below fp32
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [1, 50])
+def test_a_cache_past_32_bits(gpu, lb, rows):
+    """The pages in use lie behind 4.9 GB of others in each of k and v."""
+    s = Setup(lb, [(rows, 300), (rows, 2000 - rows)], 256, 4, 64, seed=16)
+    before = 150000
+    for name in ("k", "ks", "v", "vs"):
+        x = getattr(s, name)
+        y = torch.empty((before + x.shape[0], *x.shape[1:]), dtype=torch.uint8, device="cuda")
+        y[before:] = x
+        setattr(s, name, y)
+    s.tables, s.pages = torch.where(s.tables > 0, s.tables + before, 0), s.pages + before
+    assert before * 4 * 64 * 128 > 1 << 32
+    check_attention(lb, s, "bf16", 2)
+    k, v = (torch.randn(s.rows, 4, 256, device="cuda", generator=s.gen) for _ in range(2))
+    got_k, got_v, err = torch.empty_like(k), torch.empty_like(v), torch.zeros(1, dtype=torch.int32, device="cuda")
+    s.cache().append(s.batch(), k, v, err=err)
+    s.cache().read(s.batch(), got_k, got_v, err=err)
+    assert err.item() == 0 and torch.equal(got_k.double(), stored64(k.double())) and torch.equal(got_v.double(), stored64(v.double()))
+
+
+@pytest.mark.gpu
+def test_attention_sequences_that_share_rows_stay_in_bounds(gpu, lb):
+    """row0 that descends is against the rules: recorded, and nothing beyond the arrays is touched."""
+    H, D, G, n = 1, 64, 8, 20
+    s = Setup(lb, [(100, 1100)], D, H, 16, seed=17)
+    row0 = torch.tensor([0, 100] * n + [0, 100, 200], dtype=torch.int32, device="cuda")
+    seqs = len(row0) - 1
+    batch = lb.Kv4Batch(row0, s.slot.repeat(seqs), s.pos.repeat(seqs), 200, 100, 1200)
+    q = torch.randn(200, H * G, D, device="cuda", generator=s.gen).bfloat16()
+    out = torch.full((202, H * G, D), 9.0, dtype=torch.bfloat16, device="cuda")
+    need = s.cache().attention_workspace_bytes(batch, H * G)
+    work, err = torch.zeros(need + 4096, dtype=torch.uint8, device="cuda"), torch.zeros(1, dtype=torch.int32, device="cuda")
+    s.cache().attention(batch, q, out[1:201], 0.125, work[:need], err=err)
+    assert err.item() == BAD_BATCH and (out[0] == 9.0).all() and (out[201] == 9.0).all() and not work[need:].any()
 
 
 @pytest.mark.gpu
