@@ -304,7 +304,7 @@ __global__ void __launch_bounds__(kThreads, 1) nvfp4_matvec_kernel(MatvecArgs a)
   for (int tile = tile0; tile < tile1; tile += batch) {
     const int batch_tiles = min(batch, tile1 - tile), last_pair = first_pair(tile, group + 1);
     for (int pair = first_pair(tile, group); pair < last_pair; ++pair) {
-      float acc[2][NT][4] = {};
+      float total[2][NT][4] = {};
       for (int unit = u0; unit < u1; unit += kChunkUnits) {
         const int n_units = min(kChunkUnits, u1 - unit);
         cp_wait_but(S - 2);
@@ -323,6 +323,7 @@ __global__ void __launch_bounds__(kThreads, 1) nvfp4_matvec_kernel(MatvecArgs a)
           }
         const uint8_t* row_w = st + g * 128 + t * 16;
         const int x_off = (unit - c0) * 64;
+        float acc[2][NT][4] = {};  // of this chunk: an MMA cuts its sums off instead of rounding them, which a long chain would add up
         auto piece = [&](int p, bool here) {  // four units, this thread's being unit + 4 p + t; !here: it is not in the chunk
           uint32_t w[2][2][4], sc[2][2][2];  // codes; scales of the two groups
 #pragma unroll
@@ -369,13 +370,19 @@ __global__ void __launch_bounds__(kThreads, 1) nvfp4_matvec_kernel(MatvecArgs a)
 #pragma unroll 1
           for (int p = 0; p * 4 < n_units; ++p) piece(p, p * 4 + t < n_units);
         }
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) total[i][n][j] += acc[i][n][j];
       }
       if (c > 1 && read_pending) cluster_wait(), read_pending = false;
 #pragma unroll
       for (int i = 0; i < 2; ++i)
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-          const float(&v)[4] = acc[i][n];
+          const float(&v)[4] = total[i][n];
           const float4 s = make_float4(v[0] * inv[n][0], v[1] * inv[n][1], v[2] * inv[n][0], v[3] * inv[n][1]);
           const int at = pair * 2 + i;  // in the batch
           if (at >= batch_tiles) continue;
