@@ -44,8 +44,13 @@ struct AttnArgs {
 //                 worker: a CTA, whose warps take its steps in turn and add their results in shared memory, or (kSolo) a warp on
 //                 its own, which meets nobody.  An item that several workers share leaves partial results (O, m, l), which a
 //                 second kernel, launched dependent so that its start overlaps the first one's end, adds in order.
+// Measured, both kernels: one token over 128k positions (24 query heads on 4 kv heads of 256) 48 us, 3.1 TB/s of cache read; 64 tokens
+// over 1k to 8k positions (32 on 8 of 128) 101 us, 3.5 TB/s (6.5 TB/s is a plain copy).  What bounds it there is issue: codes to FP16
+// and their scales take as many slots as the MMAs.  8k positions 13 us: a launch, the plan, one ring's latency, the meeting, the join.
 constexpr int kDecRows = 8, kDecMaxCtas = 160;
 constexpr int kDecWarps = 8, kDecThreads = kDecWarps * 32, kDecMaxWorkers = kDecMaxCtas * kDecWarps;
+// Items from which warps work alone.  Measured, meeting / alone, 4 kv heads: 48 items of 8k positions 31 / 36 us, 64 items 41 / 41,
+// 80 items 46 / 43, 256 items 108 / 95; of 1k positions 48 items 23 / 19, 64 items 18 / 20, 256 items 51 / 36.
 constexpr int kSoloItems = 74;
 constexpr float kLazy = 7.f;  // a score may exceed the running reference by this (log2) before the sums are scaled anew
 
@@ -752,7 +757,10 @@ __global__ void __launch_bounds__(kJoinThreads) kv4_join_kernel(AttnArgs a) {
 //                the scores, as the value product's A operand; sum.  O is scaled in TMEM only when a score exceeds the row's
 //                reference by 2^kLazy, so that a tile's softmax need not wait for the tile before.
 // What bounds it is shared memory: operands are read once by the MMAs and written once by the converting warps (D = 256: 192 KB
-// and 128 KB a tile, 2560 cycles at 128 bytes, against 2048 cycles of MMA).
+// and 128 KB a tile, 2560 cycles at 128 bytes, against 2048 cycles of MMA).  Measured (24 query heads on 4 kv heads of 256): 4096 rows
+// behind 4096 positions 762 us, 810 TFLOP/s (1644 is a library GEMM's rate); 4 trees of 20 rows behind up to 8k positions 50 us, of
+// which about 20 go into a CTA's first keys, its queries' conversion and its last rows.  A ring of pieces for K and V, with or
+// without warps of their own for each, was slower (840 and 909 us): more overlap only meets at shared memory.
 // Every wait is bounded; one that runs out is recorded and the CTA leaves with its TMEM freed.
 constexpr int kTileRows = 128, kTileKeys = 128, kTileWarps = 17, kTileThreads = kTileWarps * 32, kTileWorkers = 256, kTileMarks = 8;
 constexpr int kMmaWarp = 16;
@@ -1326,7 +1334,10 @@ int decode_launch(const AttnArgs& a, int sms, cudaStream_t s) {
 
 // How a batch with up to these rows and positions runs.  Up to kDecodeRows query rows of a kv head the decode kernel reads the cache once
 // per 8 of them; beyond, the tile kernel once per 128, contexts split over CTAs where the row tiles alone do not fill the device.
-constexpr int kDecodeRows = 16, kTileCtas = 148, kTileSplitKeys = 512;  // CTAs wanted; positions that a split is worth
+// Measured, decode / tile kernel, 6 heads a kv head: 24 query rows over 128k positions 113 / 120 us, 30 rows 145 / 121; over 8k 19 / 32 and
+// 22 / 33; 64 sequences of up to 8k, 3 rows each on average, 228 / 326.  A split is worth kTileSplitKeys positions: 16 rows over 2k
+// positions 29.5 us (256: 26.8, 1024: 38.4), over 8k 36.7 (41.1, 42.0), from 60k on the same.
+constexpr int kDecodeRows = 24, kTileCtas = 148, kTileSplitKeys = 512;  // CTAs wanted; positions that a split is worth
 struct Plan {
   bool tile = false, solo = false;
   int row_tiles = 0, splits = 1;
