@@ -758,8 +758,8 @@ __global__ void __launch_bounds__(kJoinThreads) kv4_join_kernel(AttnArgs a) {
 //                reference by 2^kLazy, so that a tile's softmax need not wait for the tile before.
 // What bounds it is shared memory: operands are read once by the MMAs and written once by the converting warps (D = 256: 192 KB
 // and 128 KB a tile, 2560 cycles at 128 bytes, against 2048 cycles of MMA).  Measured (24 query heads on 4 kv heads of 256): 4096 rows
-// behind 4096 positions 762 us, 810 TFLOP/s (1644 is a library GEMM's rate); 4 trees of 20 rows behind up to 8k positions 50 us, of
-// which about 20 go into a CTA's first keys, its queries' conversion and its last rows.  A ring of pieces for K and V, with or
+// behind 4096 positions 757 us, 817 TFLOP/s (1644 is a library GEMM's rate); 4 trees of 20 rows behind up to 8k positions 48 us, of
+// which nearly 20 go into a CTA's first keys, its queries' conversion and its last rows.  A ring of pieces for K and V, with or
 // without warps of their own for each, was slower (840 and 909 us): more overlap only meets at shared memory.
 // Every wait is bounded; one that runs out is recorded and the CTA leaves with its TMEM freed.
 constexpr int kTileRows = 128, kTileKeys = 128, kTileWarps = 17, kTileThreads = kTileWarps * 32, kTileWorkers = 256, kTileMarks = 8;
@@ -872,9 +872,9 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv4_tile_kernel(AttnArgs a, i
   const int all_see = a.b.anc ? sq.pos : sq.pos + f0 / G + 1;                     // every row sees at least these
   const int tiles = (keys + kTileKeys - 1) / kTileKeys;
   const int t0 = int((long long)tiles * blockIdx.z / splits), nt = int((long long)tiles * (blockIdx.z + 1) / splits) - t0;
-  float* part = a.parts + ((size_t(index) * H + h) * splits + blockIdx.z) * tile_part_floats(D);
+  auto partial = [&] { return a.parts + ((size_t(index) * H + h) * splits + blockIdx.z) * tile_part_floats(D); };
   if (nt == 0) {  // (more splits than tiles)
-    if (tid < kTileRows) part[kTileRows * D + tid] = -INFINITY, part[kTileRows * D + kTileRows + tid] = 0.f;
+    if (tid < kTileRows) partial()[kTileRows * D + tid] = -INFINITY, partial()[kTileRows * D + kTileRows + tid] = 0.f;
     return;
   }
   if (warp == kMmaWarp) {
@@ -889,23 +889,26 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv4_tile_kernel(AttnArgs a, i
     const int sub = lane / kLanes, piece = lane % kLanes;
     for (int r0 = warp * kRowsAtOnce * kFly; r0 < kTileRows; r0 += kTileWarps * kRowsAtOnce * kFly) {
       uint4 w[kFly];
+      const T* src[kFly];
 #pragma unroll
-      for (int i = 0; i < kFly; ++i) {
-        const int r = r0 + i * kRowsAtOnce + sub, f = f0 + r;
-        w[i] = make_uint4(0, 0, 0, 0);
-        if (r < kTileRows && f < R) {
-          const T* src = static_cast<const T*>(a.q.p) + (sq.row0 + f / G) * a.q.row + (h * G + f % G) * a.q.head + piece * 8;
-          if (a.q_vec) {
-            w[i] = *reinterpret_cast<const uint4*>(src);
-          } else {
-            const uint16_t* e = reinterpret_cast<const uint16_t*>(src);
-            w[i] = make_uint4(e[0] | uint32_t(e[1]) << 16, e[2] | uint32_t(e[3]) << 16, e[4] | uint32_t(e[5]) << 16, e[6] | uint32_t(e[7]) << 16);
-          }
+      for (int i = 0; i < kFly; ++i) {  // (rows past the last read the last one's, so that all loads are under way together)
+        const int f = min(f0 + r0 + i * kRowsAtOnce + sub, R - 1);
+        src[i] = static_cast<const T*>(a.q.p) + (sq.row0 + f / G) * a.q.row + (h * G + f % G) * a.q.head + piece * 8;
+      }
+      if (a.q_vec) {
+#pragma unroll
+        for (int i = 0; i < kFly; ++i) w[i] = *reinterpret_cast<const uint4*>(src[i]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < kFly; ++i) {
+          const uint16_t* e = reinterpret_cast<const uint16_t*>(src[i]);
+          w[i] = make_uint4(e[0] | uint32_t(e[1]) << 16, e[2] | uint32_t(e[3]) << 16, e[4] | uint32_t(e[5]) << 16, e[6] | uint32_t(e[7]) << 16);
         }
       }
 #pragma unroll
       for (int i = 0; i < kFly; ++i) {
         const int r = r0 + i * kRowsAtOnce + sub;
+        if (f0 + r >= R) w[i] = make_uint4(0, 0, 0, 0);
         uint32_t top2 = __vmaxu2(__vmaxu2(w[i].x & 0x7fff7fffu, w[i].y & 0x7fff7fffu), __vmaxu2(w[i].z & 0x7fff7fffu, w[i].w & 0x7fff7fffu));
 #pragma unroll
         for (int o = 1; o < kLanes; o <<= 1) top2 = __vmaxu2(top2, __shfl_xor_sync(0xffffffffu, top2, o));
@@ -1199,30 +1202,45 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv4_tile_kernel(AttnArgs a, i
     l = row_max[nt & 1][0][r] + row_max[nt & 1][1][r];
     if (ok && wait(&pv_done[(nt - 1) & 1], (nt - 1) >> 1, kDevWaitTmemFull)) {
       tc_fence_after();
+      float* part = partial();
       const bool empty = m == -INFINITY && l == 0.f;
       const float scale = empty ? 0.f : a.c.v_scale / l;
       const int row = sq.row0 + (real ? i_row : 0), head = h * G + (real ? f % G : 0);
       T* to = static_cast<T*>(a.out.p) + row * a.out.row + head * a.out.head;
+      // O by rows is what a thread holds; the operands' memory, which no MMA reads any more, turns it for whole lines
+      constexpr int kStage = D + 16;  // bytes of half a row, padded against bank conflicts
+      uint8_t* stage = ks + warp * (32 * kStage);
 #pragma unroll 1
       for (int c = half * (D / 64); c < (half + 1) * (D / 64); ++c) {
         uint32_t x[32];
         tmem_ld32(lane_addr + kOcol + c * 32, x);
         tmem_ld_wait();
-        if (!real) continue;
-        if (splits > 1) {
+        if (splits > 1) {  // [dims / 4][row][4]
 #pragma unroll
-          for (int j = 0; j < 32; j += 4) *reinterpret_cast<uint4*>(part + size_t(r) * D + c * 32 + j) = make_uint4(x[j], x[j + 1], x[j + 2], x[j + 3]);
+          for (int j = 0; j < 32; j += 4)
+            *reinterpret_cast<uint4*>(part + (size_t(c * 8 + j / 4) * kTileRows + r) * 4) = make_uint4(x[j], x[j + 1], x[j + 2], x[j + 3]);
         } else if (a.out_vec) {
 #pragma unroll
           for (int j = 0; j < 32; j += 8) {
             T e[8];
 #pragma unroll
             for (int y = 0; y < 8; ++y) e[y] = from_f32<T>(empty ? 0.f : __uint_as_float(x[j + y]) * scale);
-            *reinterpret_cast<uint4*>(to + c * 32 + j) = *reinterpret_cast<const uint4*>(e);
+            *reinterpret_cast<uint4*>(stage + lane * kStage + (c - half * (D / 64)) * 64 + j * 2) = *reinterpret_cast<const uint4*>(e);
           }
-        } else {
+        } else if (real) {
 #pragma unroll
           for (int j = 0; j < 32; ++j) to[c * 32 + j] = from_f32<T>(empty ? 0.f : __uint_as_float(x[j]) * scale);
+        }
+      }
+      if (splits == 1 && a.out_vec) {
+        __syncwarp();
+        constexpr int kLanes = D / 16, kAtOnce = 32 / kLanes;  // lanes of half a row
+        T* out = static_cast<T*>(a.out.p) + half * (D / 2);
+        for (int i = lane / kLanes; i < 32; i += kAtOnce) {
+          const int fi = f0 + (warp & 3) * 32 + i;
+          if (fi >= R) break;
+          T* dst = out + (sq.row0 + fi / G) * a.out.row + (h * G + fi % G) * a.out.head;
+          reinterpret_cast<uint4*>(dst)[lane % kLanes] = *reinterpret_cast<const uint4*>(stage + i * kStage + lane % kLanes * 16);
         }
       }
       if (half == 0) {
@@ -1243,51 +1261,78 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv4_tile_kernel(AttnArgs a, i
 template <typename T, int D>
 __global__ void __launch_bounds__(256) kv4_tile_join_kernel(AttnArgs a, int splits, int row_tiles) {
   pdl_sync();  // first statement: see common.cuh
-  const int lane = threadIdx.x & 31, G = a.q_heads / a.c.kv_heads, H = a.c.kv_heads, h = blockIdx.y;
-  const int r = blockIdx.x * 8 + (threadIdx.x >> 5);  // packed row * G + head of the group
-  const int row = r / G, head = h * G + r % G;
-  if (row >= a.b.rows) return;
-  // the sequence and its first tile
-  int before = 0, seq = -1, tile0 = 0;
-  for (int s0 = 0; s0 < a.b.seqs && seq < 0; s0 += 32) {
-    const int s = s0 + lane;
-    Kv4Seq q{0, 0, 0, 0, false};
-    if (s < a.b.seqs) q = kv4_seq(a.c, a.b, s);
-    const int n = q.ok ? (q.n * G + kTileRows - 1) / kTileRows : 0;
-    int end = n;
+  __shared__ int at[8];  // of the block's rows: tile * kTileRows + row of the tile; -1: none
+  const int tid = threadIdx.x, lane = tid & 31, G = a.q_heads / a.c.kv_heads, H = a.c.kv_heads, h = blockIdx.y;
+  // ---- a warp a row (packed row * G + head of the group): the sequence and its first tile
+  {
+    const int r = blockIdx.x * 8 + (tid >> 5), row = r / G;
+    int before = 0, seq = -1, tile0 = 0;
+    for (int s0 = 0; s0 < a.b.seqs && seq < 0; s0 += 32) {
+      const int s = s0 + lane;
+      Kv4Seq q{0, 0, 0, 0, false};
+      if (s < a.b.seqs) q = kv4_seq(a.c, a.b, s);
+      const int n = q.ok ? (q.n * G + kTileRows - 1) / kTileRows : 0;
+      int end = n;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int v = __shfl_up_sync(0xffffffffu, end, o);
-      if (lane >= o) end += v;
+      for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, end, o);
+        if (lane >= o) end += v;
+      }
+      end += before;
+      const unsigned mine = __ballot_sync(0xffffffffu, q.ok && row >= q.row0 && row < q.row0 + q.n);
+      if (mine) {
+        seq = s0 + __ffs(mine) - 1;
+        tile0 = __shfl_sync(0xffffffffu, end - n, __ffs(mine) - 1);
+      }
+      before = __shfl_sync(0xffffffffu, end, 31);
     }
-    end += before;
-    const unsigned mine = __ballot_sync(0xffffffffu, q.ok && row >= q.row0 && row < q.row0 + q.n);
-    if (mine) {
-      seq = s0 + __ffs(mine) - 1;
-      tile0 = __shfl_sync(0xffffffffu, end - n, __ffs(mine) - 1);
-    }
-    before = __shfl_sync(0xffffffffu, end, 31);
+    int f = 0;
+    if (seq >= 0) f = (row - a.b.row0[seq]) * G + r % G;
+    // (more tiles than rows have: sequences that share rows, against the batch's rules)
+    if (lane == 0) at[tid >> 5] = seq >= 0 && row < a.b.rows && tile0 + f / kTileRows < row_tiles ? (tile0 + f / kTileRows) * kTileRows + f % kTileRows : -1;
   }
-  if (seq < 0) return;
-  const int f = (row - a.b.row0[seq]) * G + r % G, in = f % kTileRows;
-  if (tile0 + f / kTileRows >= row_tiles) return;  // (sequences that share rows, against the batch's rules: more tiles than rows have)
-  const float* parts = a.parts + (size_t(tile0 + f / kTileRows) * H + h) * splits * tile_part_floats(D);
+  __syncthreads();
+  // ---- a thread four dims of a row: eight neighbouring rows' are 128 bytes of a partial result
+  const int mine = at[tid & 7], r = blockIdx.x * 8 + (tid & 7), in = mine & (kTileRows - 1);
+  if (mine < 0) return;
+  const float* parts = a.parts + (size_t(mine / kTileRows) * H + h) * splits * tile_part_floats(D);
   float mm = -INFINITY;
   for (int s = 0; s < splits; ++s) mm = fmaxf(mm, parts[s * tile_part_floats(D) + kTileRows * D + in]);
-  float l = 0.f, o[D / 32] = {};
+  constexpr int kEach = D == 256 ? 2 : 1;
+  const int quad = tid >> 3;
+  if (quad >= D / 4) return;
+  float l = 0.f;
+  float4 o[kEach] = {};
+#pragma unroll 4
   for (int s = 0; s < splits; ++s) {
     const float* p = parts + s * tile_part_floats(D);
     const float ps = p[kTileRows * D + kTileRows + in], w = part_weight(p[kTileRows * D + in], ps, mm);
     if (w == 0.f) continue;  // (a split without keys has written no O)
     l = fmaf(ps, w, l);
 #pragma unroll
-    for (int j = 0; j < D / 32; ++j) o[j] = fmaf(p[size_t(in) * D + j * 32 + lane], w, o[j]);
+    for (int j = 0; j < kEach; ++j) {
+      const float4 x = *reinterpret_cast<const float4*>(p + (size_t(quad + j * 32) * kTileRows + in) * 4);
+      o[j].x = fmaf(x.x, w, o[j].x), o[j].y = fmaf(x.y, w, o[j].y), o[j].z = fmaf(x.z, w, o[j].z), o[j].w = fmaf(x.w, w, o[j].w);
+    }
   }
   const bool empty = mm == -INFINITY && l == 0.f;
+  const int row = r / G, head = h * G + r % G;
   T* to = static_cast<T*>(a.out.p) + row * a.out.row + head * a.out.head;
 #pragma unroll
-  for (int j = 0; j < D / 32; ++j) to[j * 32 + lane] = from_f32<T>(empty ? 0.f : o[j] / l * a.c.v_scale);
-  if (a.lse && lane == 0) a.lse[size_t(row) * a.q_heads + head] = empty ? -INFINITY : (mm + log2f(l) - kPShift) * kLn2;
+  for (int j = 0; j < kEach; ++j) {
+    const float x[4] = {o[j].x, o[j].y, o[j].z, o[j].w};
+    T e[4];
+#pragma unroll
+    for (int y = 0; y < 4; ++y) e[y] = from_f32<T>(empty ? 0.f : x[y] / l * a.c.v_scale);
+    T* dst = to + (quad + j * 32) * 4;
+    if (a.out_vec) {
+      *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(e);
+    } else {
+#pragma unroll
+      for (int y = 0; y < 4; ++y) dst[y] = e[y];
+    }
+  }
+  if (a.lse && quad == 0) a.lse[size_t(row) * a.q_heads + head] = empty ? -INFINITY : (mm + log2f(l) - kPShift) * kLn2;
 }
 
 template <typename T, int D>
@@ -1336,7 +1381,7 @@ int decode_launch(const AttnArgs& a, int sms, cudaStream_t s) {
 // per 8 of them; beyond, the tile kernel once per 128, contexts split over CTAs where the row tiles alone do not fill the device.
 // Measured, decode / tile kernel, 6 heads a kv head: 24 query rows over 128k positions 113 / 120 us, 30 rows 145 / 121; over 8k 19 / 32 and
 // 22 / 33; 64 sequences of up to 8k, 3 rows each on average, 228 / 326.  A split is worth kTileSplitKeys positions: 16 rows over 2k
-// positions 29.5 us (256: 26.8, 1024: 38.4), over 8k 36.7 (41.1, 42.0), from 60k on the same.
+// positions 27.5 us (256: 26.8, 1024: 38.4), over 8k 34.3 (41.1, 42.0), from 60k on the same.
 constexpr int kDecodeRows = 24, kTileCtas = 148, kTileSplitKeys = 512;  // CTAs wanted; positions that a split is worth
 struct Plan {
   bool tile = false, solo = false;
