@@ -687,8 +687,9 @@ int ling_b200_draft_head_run_sparse(ling_b200_draft_head* h, int session, const 
  * paged KV cache, attention over it.  Unlike the _host entry points these take DEVICE pointers and only enqueue on `stream` (a
  * cudaStream_t; NULL = the default stream): they allocate nothing, wait for nothing and may be captured into a graph.  All
  * pointers and the stream belong to `device`, which need not be the calling thread's current one.  A call that is refused
- * launches nothing.  `err`, where there is one, is a device word or NULL: the first error that the kernels find (a page id out of
- * range, a batch outside its bounds) is recorded there (it is never cleared by the library), the positions concerned are skipped. */
+ * launches nothing.  `err`, where there is one, is a device word or NULL: the first error that the kernels find (5: a page id out
+ * of range, 8: a batch outside its bounds, below 5: a bounded wait that ran out) is recorded there (it is never cleared by the
+ * library), the positions concerned are skipped. */
 enum { LING_B200_F32 = 0, LING_B200_BF16 = 1, LING_B200_F16 = 2 }; /* element types */
 
 /* y[m][n] = alpha * sum_k x[m][k] * w[n][k] (or += with accumulate) for M rows, 1 <= M <= 32; w as ling_b200_quantize_nvfp4_host leaves it

@@ -372,6 +372,7 @@ extern "C" int ling_b200_kv4_append(int device, const ling_b200_kv4* cache, cons
     set_error("kv4_append: element types are LING_B200_F32, _BF16 and _F16");
     return LING_B200_ERR_ARG;
   }
+  if (batch->rows == 0) return LING_B200_OK;  // (arrays without rows may have no address)
   const int D = cache->head_dim;
   if (!kv4_rows_ok(k, type, cache->kv_heads, D, who, "k") || !kv4_rows_ok(v, type, cache->kv_heads, D, who, "v")) return LING_B200_ERR_ARG;
   if (!q != !q_out || (q && (q_heads < 1 || q_heads > 1024 || !kv4_rows_ok(q, type, q_heads, D, who, "q") || !kv4_out_ok(q_out, type, batch->rows, q_heads, D, who, "q_out")))) {
@@ -382,7 +383,6 @@ extern "C" int ling_b200_kv4_append(int device, const ling_b200_kv4* cache, cons
     set_error("kv4_append: rotary_dim must be even and at most head_dim, theta positive and finite");
     return LING_B200_ERR_ARG;
   }
-  if (batch->rows == 0) return LING_B200_OK;
   DeviceGuard guard;
   int sms = 0;
   if (const int r = enter_device(guard, device, g_devices, g_mutex, [] { return LING_B200_OK; }, &sms)) return r;
@@ -401,10 +401,10 @@ extern "C" int ling_b200_kv4_read(int device, const ling_b200_kv4* cache, const 
     set_error("kv4_read: a type and k or v expected");
     return LING_B200_ERR_ARG;
   }
+  if (batch->rows == 0) return LING_B200_OK;
   if ((k && !kv4_out_ok(k, type, batch->rows, cache->kv_heads, cache->head_dim, who, "k")) ||
       (v && !kv4_out_ok(v, type, batch->rows, cache->kv_heads, cache->head_dim, who, "v")))
     return LING_B200_ERR_ARG;
-  if (batch->rows == 0) return LING_B200_OK;
   DeviceGuard guard;
   int sms = 0;
   if (const int r = enter_device(guard, device, g_devices, g_mutex, [] { return LING_B200_OK; }, &sms)) return r;

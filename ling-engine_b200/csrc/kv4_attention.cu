@@ -1451,6 +1451,7 @@ extern "C" int ling_b200_kv4_attention(int device, const ling_b200_kv4* cache, c
     set_error("kv4_attention: queries are LING_B200_BF16 or LING_B200_F16");
     return LING_B200_ERR_ARG;
   }
+  if (batch->rows == 0) return LING_B200_OK;  // (arrays without rows may have no address)
   if (!kv4_rows_ok(q, type, q_heads, cache->head_dim, who, "q") || !kv4_out_ok(out, type, batch->rows, q_heads, cache->head_dim, who, "out"))
     return LING_B200_ERR_ARG;
   if (!std::isfinite(scale) || !aligned(lse, 4) || !aligned(err, 4)) {
@@ -1467,7 +1468,7 @@ extern "C" int ling_b200_kv4_attention(int device, const ling_b200_kv4* cache, c
     set_error("kv4_attention: a 16-byte aligned workspace of " + std::to_string(need) + " bytes expected");
     return LING_B200_ERR_ARG;
   }
-  if (batch->rows == 0 || batch->max_rows == 0) return LING_B200_OK;
+  if (batch->max_rows == 0) return LING_B200_OK;
   DeviceGuard guard;
   int sms = 0;
   if (const int r = enter_device(guard, device, g_devices, g_mutex, attention_init, &sms)) return r;

@@ -146,6 +146,7 @@ def test_other_refusals(lb):
     assert lb.lib().ling_b200_kv4_attention_workspace(C.byref(ok[0]), C.byref(ok[1]), 3) == 0
     # an empty call is a call: nothing is launched, no device is needed
     assert calls(lb, c_cache(lb), c_batch(lb, rows=0, max_rows=0)) == (lb.OK,) * 3
+    assert calls(lb, c_cache(lb), c_batch(lb, rows=0, max_rows=0), rows=(0, 256, 128), q=(0, 512, 128), out=(0, 512, 128), wsp=0) == (lb.OK,) * 3
 
 
 def test_host_arrays_are_refused(lb):
