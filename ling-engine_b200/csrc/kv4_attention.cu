@@ -1058,7 +1058,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv4_tile_kernel(AttnArgs a, i
       ask(v_unit, vs_unit, vec, vc);
       if (w < 4) bad_keys[(t + 3) % kTileMarks][w] = 0, nan_keys[(t + 3) % kTileMarks][w] = 0;  // (last used five tiles ago)
       if (t + 1 < nt) {  // K(t + 1), where K(t) was
-        ok = wait(&qk_done[t & 1], t >> 1, kDevWaitEmpty);
+        ok = __all_sync(0xffffffffu, wait(&qk_done[t & 1], t >> 1, kDevWaitEmpty));  // (a warp gives up as one)
         if (!ok) break;
         mark_bad(t + 1, vec1);
         convert(ks, kc);
@@ -1076,7 +1076,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv4_tile_kernel(AttnArgs a, i
             vc.s[u] = 0;
           }
       }
-      ok = t == 0 || wait(&pv_done[(t - 1) & 1], (t - 1) >> 1, kDevWaitEmpty);  // V(t), where V(t - 1) was
+      ok = __all_sync(0xffffffffu, t == 0 || wait(&pv_done[(t - 1) & 1], (t - 1) >> 1, kDevWaitEmpty));  // V(t), where V(t - 1) was
       if (!ok) break;
       convert(vs, vc);
       publish(&v_full);
@@ -1200,7 +1200,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv4_tile_kernel(AttnArgs a, i
     row_max[nt & 1][half][r] = l;
     ok = meet_all(ok);
     l = row_max[nt & 1][0][r] + row_max[nt & 1][1][r];
-    if (ok && wait(&pv_done[(nt - 1) & 1], (nt - 1) >> 1, kDevWaitTmemFull)) {
+    if (__all_sync(0xffffffffu, ok && wait(&pv_done[(nt - 1) & 1], (nt - 1) >> 1, kDevWaitTmemFull))) {
       tc_fence_after();
       float* part = partial();
       const bool empty = m == -INFINITY && l == 0.f;
