@@ -696,8 +696,9 @@ enum { LING_B200_F32 = 0, LING_B200_BF16 = 1, LING_B200_F16 = 2 }; /* element ty
  * (values [N][K/2], scales [N][K/16], K % 16 == 0; alpha carries the tensor scale).  x [M][ldx], y [M][ldy] of any two of the
  * types above, ldx >= K, ldy >= N in elements; y must not overlap x.  x stays in its type (fp32 included: no activation
  * quantizer, unlike ling_b200_prefill_gemm_nvfp4_host), sums are fp32, each y is rounded once.  A row's result does
- * not depend on what the other rows hold.  values on an 8-byte boundary.  K up to
- * 17408 and beyond; ERR_UNSUPPORTED where eight rows' activations no longer fit a cluster's shared memory (K above about 60000). */
+ * not depend on what the other rows hold.  values on an 8-byte boundary.
+ * K up to 57344 (up to four 16-bit or two fp32 rows: 114688, one 16-bit row: 462848); ERR_UNSUPPORTED where the activations of eight columns
+ * (a 16-bit row is one, an fp32 row two), or of as many as there are, no longer fit a cluster's shared memory. */
 int ling_b200_nvfp4_matvec(int device, const void* x, int x_type, long long ldx, int M, const uint8_t* values, const uint8_t* scales,
                            float alpha, int N, int K, void* y, int y_type, long long ldy, int accumulate, void* stream);
 

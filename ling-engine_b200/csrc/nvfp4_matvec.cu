@@ -473,6 +473,12 @@ int init_all(int device) {
   return init_type<__half>(g_clusters[device]);
 }
 
+// Whether `cols` columns of K activations fit a cluster of 8 CTAs beside the sums and the shortest rings: what every plan can fall back to.
+bool fits(int K, int cols) {
+  const long long chunks = ((long long)K + kUnit * kChunkUnits - 1) / (kUnit * kChunkUnits), cta_chunks = (chunks + 7) / 8;
+  return cta_chunks * kChunkUnits * 64 * cols <= kSmem - kSumBlocks * 512 - 2 * kWarps * kStageBytes;
+}
+
 // CTAs and warps that share K: the split with the least estimated time.  A warp's stage takes its share of the SM's part of HBM (4736
 // bytes at 5.5 a nanosecond), or the loaded latency of about 2 us over the stages in flight, or its instructions (about 700 ns and
 // 150 a column tile beyond the first); a meeting costs about 0.7 us, of a cluster's CTAs 2 us.  false: `cols` columns of activations (in
@@ -513,7 +519,8 @@ int matvec_launch(MatvecArgs a, const Split& split, cudaStream_t s) {
   LB_LAUNCH("nvfp4_matvec_kernel");
   return LING_B200_OK;
 }
-// As many rows a launch as their activations fit beside the weights' rings (at K = 5120 all of them, at 17408 19 columns).
+// As many rows a launch as their activations fit beside the weights' rings: at K = 5120 32 columns, at 17408 25 (in 4 tiles; the rows left
+// over are launches of their own, which read the weights again).
 template <typename TX>
 int matvec_rows(MatvecArgs a, int device, cudaStream_t s) {
   constexpr int kCols = sizeof(TX) == 4 ? 2 : 1;
@@ -523,13 +530,7 @@ int matvec_rows(MatvecArgs a, int device, cudaStream_t s) {
     Split split;
     int nt = 4, left = (a.M - m) * kCols;
     while (nt > 1 && left <= 4 * nt) nt /= 2;
-    while (!choose_split(g_clusters[device], a.N, a.K, nt, std::min(left, 8 * nt), &split)) {
-      if (nt == 1) {
-        set_error("nvfp4_matvec: K = " + std::to_string(a.K) + " is beyond the activations' shared memory");
-        return LING_B200_ERR_UNSUPPORTED;
-      }
-      nt /= 2;
-    }
+    while (!choose_split(g_clusters[device], a.N, a.K, nt, std::min(left, 8 * nt), &split)) nt /= 2;  // (8 columns fit)
     rows = std::min(a.M - m, 8 * nt / kCols);
     b.x = x + m * a.ldx, b.M = rows, b.y = static_cast<uint8_t*>(a.y) + m * a.ldy * type_size(a.y_type);
     const int r = nt == 1 ? matvec_launch<TX, 1>(b, split, s) : nt == 2 ? matvec_launch<TX, 2>(b, split, s) : matvec_launch<TX, 4>(b, split, s);
@@ -554,6 +555,10 @@ extern "C" int ling_b200_nvfp4_matvec(int device, const void* x, int x_type, lon
       !d4::aligned(x, d4::type_size(x_type)) || !d4::aligned(y, d4::type_size(y_type)) || !d4::aligned(values, 8)) {
     set_error("nvfp4_matvec: bad argument (1 <= M <= 32, K a multiple of 16, ldx >= K, ldy >= N, values on an 8-byte boundary)");
     return LING_B200_ERR_ARG;
+  }
+  if (!fits(K, std::min(8, M * (x_type == LING_B200_F32 ? 2 : 1)))) {
+    set_error("nvfp4_matvec: K = " + std::to_string(K) + " is beyond the activations' shared memory");
+    return LING_B200_ERR_UNSUPPORTED;
   }
   d4::DeviceGuard guard;
   int sms = 0;

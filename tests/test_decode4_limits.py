@@ -1,0 +1,34 @@
+"""Calls at the limits of the operators of a decode layer in 4 bits: sizes at which an index would leave 32 bits, batches against the
+rules, contexts so long that a sum's roundings add up, values on a rounding's border.  Refusals are checked without a GPU."""
+import ctypes as C
+import math
+
+import pytest
+
+torch = pytest.importorskip("torch")
+
+from test_decode4 import c_batch, c_cache, calls, matvec_case, _p  # noqa: E402
+
+
+# ------------------------------------------------------------------------------------------------ refusals, without a GPU
+def matvec_status(lb, M, N, K, xt):
+    fn = lb.lib().ling_b200_nvfp4_matvec
+    fn.argtypes = lb._MATVEC_ARGS
+    return fn(0, _p(), xt, K, M, _p(2), _p(3), 1.0, N, K, _p(4), lb.F32, N, 0, None)
+
+
+@pytest.mark.parametrize("K", [57344 + 16, 1 << 20, 1 << 25, 34000000, (1 << 31) - 16])
+def test_matvec_refuses_activations_beyond_shared_memory(lb, K):
+    """Before any plan is made: at K = 2^25 the activations of 32 columns are 2^31 bytes."""
+    for M, xt in ((8, lb.BF16), (32, lb.BF16), (32, lb.F16), (4, lb.F32), (32, lb.F32)):
+        assert matvec_status(lb, M, 8, K, xt) == lb.ERR_UNSUPPORTED and "shared memory" in lb.last_error()
+    if K > 462848:
+        assert matvec_status(lb, 1, 8, K, lb.BF16) == lb.ERR_UNSUPPORTED
+
+
+# ------------------------------------------------------------------------------------------------ products
+@pytest.mark.gpu
+@pytest.mark.parametrize("M,K,xt", [(8, 57344, "bf16"), (32, 57344, "f16"), (5, 57328, "f32"), (1, 462848, "bf16"), (2, 230016, "f16")])
+def test_matvec_longest_reductions(gpu, lb, M, K, xt):
+    """The longest K that a row count takes, and launches of eight columns each where there are more."""
+    matvec_case(lb, M, 100, K, xt, "f32")
