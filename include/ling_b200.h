@@ -696,7 +696,7 @@ enum { LING_B200_F32 = 0, LING_B200_BF16 = 1, LING_B200_F16 = 2 }; /* element ty
  * (values [N][K/2], scales [N][K/16], K % 16 == 0; alpha carries the tensor scale).  x [M][ldx], y [M][ldy] of any two of the
  * types above, ldx >= K, ldy >= N in elements; y must not overlap x.  x stays in its type (fp32 included: no activation
  * quantizer, unlike ling_b200_prefill_gemm_nvfp4_host), sums are fp32, each y is rounded once.  A row's result does
- * not depend on what the other rows hold.  values on an 8-byte boundary.
+ * not depend on what the other rows hold.  values on an 8-byte boundary.  N up to 2^31 - 32;
  * K up to 57344 (up to four 16-bit or two fp32 rows: 114688, one 16-bit row: 462848); ERR_UNSUPPORTED where the activations of eight columns
  * (a 16-bit row is one, an fp32 row two), or of as many as there are, no longer fit a cluster's shared memory. */
 int ling_b200_nvfp4_matvec(int device, const void* x, int x_type, long long ldx, int M, const uint8_t* values, const uint8_t* scales,

@@ -551,7 +551,8 @@ extern "C" int ling_b200_nvfp4_matvec(int device, const void* x, int x_type, lon
     set_error("nvfp4_matvec: element types are LING_B200_F32, _BF16 and _F16");
     return LING_B200_ERR_ARG;
   }
-  if (!x || !values || !scales || !y || M < 1 || M > 32 || N < 1 || K < 16 || K % 16 != 0 || ldx < K || ldy < N ||
+  constexpr int kMaxN = 0x7fffffff - 31;  // (the kernel counts rows in pairs of 16-row tiles)
+  if (!x || !values || !scales || !y || M < 1 || M > 32 || N < 1 || N > kMaxN || K < 16 || K % 16 != 0 || ldx < K || ldy < N ||
       !d4::aligned(x, d4::type_size(x_type)) || !d4::aligned(y, d4::type_size(y_type)) || !d4::aligned(values, 8)) {
     set_error("nvfp4_matvec: bad argument (1 <= M <= 32, K a multiple of 16, ldx >= K, ldy >= N, values on an 8-byte boundary)");
     return LING_B200_ERR_ARG;

@@ -26,6 +26,11 @@ def test_matvec_refuses_activations_beyond_shared_memory(lb, K):
         assert matvec_status(lb, 1, 8, K, lb.BF16) == lb.ERR_UNSUPPORTED
 
 
+def test_matvec_refuses_rows_of_weights_beyond_32_bits(lb):
+    for N in ((1 << 31) - 1, (1 << 31) - 31):
+        assert matvec_status(lb, 1, N, 16, lb.BF16) == lb.ERR_ARG and lb.last_error()
+
+
 # ------------------------------------------------------------------------------------------------ products
 @pytest.mark.gpu
 @pytest.mark.parametrize("M,K,xt", [(8, 57344, "bf16"), (32, 57344, "f16"), (5, 57328, "f32"), (1, 462848, "bf16"), (2, 230016, "f16")])
