@@ -715,8 +715,8 @@ typedef struct ling_b200_kv4 {
   float k_scale, v_scale;
 } ling_b200_kv4;
 /* The packed rows of a call: rows row0[s] .. row0[s+1] are sequence s, its row i stands at position pos[s] + i of the slot's table
- * (ragged, a sequence may have none; rows from row0[seqs] on are padding and are left as they were).  row0 does not descend.  Device arrays; the bounds
- * are the host's: a sequence outside them is skipped and recorded in err. */
+ * (ragged, a sequence may have none; rows from row0[seqs] on are padding and are left as they were).  Device arrays; the bounds
+ * are the host's: a sequence outside them is skipped and recorded in err, and so is the whole batch if row0 descends. */
 typedef struct ling_b200_kv4_batch {
   const int *row0, *slot, *pos; /* [seqs + 1], [seqs], [seqs] */
   const int* rope_pos;          /* [rows] the rotary position of a row, or NULL: its position (a tree's rows: pos + depth) */

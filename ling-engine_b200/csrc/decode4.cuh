@@ -175,13 +175,17 @@ inline bool rows_vec(const ling_b200_rows& r, int type) {
 __device__ __forceinline__ size_t kv4_vector(const ling_b200_kv4& c, int page, int h, int tok) {
   return (size_t(page) * c.kv_heads + h) * c.page_tokens + tok;
 }
-// The sequence of packed row r (all lanes of a warp together, any number of sequences), or -1 behind the last sequence.
+// The sequence of packed row r (all lanes of a warp together, any number of sequences); -1: no sequence has it; -2: row0 descends, so
+// that it could lie in several, or be counted to one that does not hold it.
 __device__ __forceinline__ int kv4_find_seq(const int* __restrict__ row0, int seqs, int r) {
   int n = 0;  // sequences that end at or before r
+  bool down = false;
   for (int s = 0; s < seqs; s += 32) {
-    const int i = s + int(threadIdx.x & 31);
-    n += __popc(__ballot_sync(0xffffffffu, i < seqs && row0[i + 1] <= r));
+    const int i = s + int(threadIdx.x & 31), begin = i < seqs ? row0[i] : 0, end = i < seqs ? row0[i + 1] : 0;
+    n += __popc(__ballot_sync(0xffffffffu, i < seqs && end <= r));
+    down |= end < begin;
   }
+  if (__any_sync(0xffffffffu, down)) return -2;
   return n < seqs && row0[n] <= r ? n : -1;
 }
 struct Kv4Seq {

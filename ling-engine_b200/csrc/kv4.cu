@@ -110,11 +110,12 @@ struct RowAt {
 };
 constexpr int kChunk = kThreads / 32;  // rows of a block at most
 
-// By warp: row r's place.  The error of a row whose sequence or page is out of bounds is recorded here.
+// By warp: row r's place.  The error of a row whose sequence or page is out of bounds, or whose batch's row0 descends, is recorded here.
 __device__ __forceinline__ RowAt row_at(const ling_b200_kv4& c, const ling_b200_kv4_batch& b, int r, int* err) {
   RowAt at{0, 0, 0};
   const int s = kv4_find_seq(b.row0, b.seqs, r);
-  if (s < 0) return at;  // padding behind the last sequence
+  if (s == -2 && (threadIdx.x & 31) == 0) dev_fail(err, kDevBadBatch);
+  if (s < 0) return at;  // padding behind the last sequence, or a batch against the rules
   const Kv4Seq q = kv4_seq(c, b, s);
   at.pos = q.pos + r - q.row0;
   if (q.ok) {

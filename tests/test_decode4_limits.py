@@ -1,13 +1,10 @@
 """Calls at the limits of the operators of a decode layer in 4 bits: sizes at which an index would leave 32 bits, batches against the
 rules, contexts so long that a sum's roundings add up, values on a rounding's border.  Refusals are checked without a GPU."""
-import ctypes as C
-import math
-
 import pytest
 
 torch = pytest.importorskip("torch")
 
-from test_decode4 import c_batch, c_cache, calls, matvec_case, _p  # noqa: E402
+from test_decode4 import BAD_BATCH, Setup, matvec_case, _p  # noqa: E402
 
 
 # ------------------------------------------------------------------------------------------------ refusals, without a GPU
@@ -37,3 +34,23 @@ def test_matvec_refuses_rows_of_weights_beyond_32_bits(lb):
 def test_matvec_longest_reductions(gpu, lb, M, K, xt):
     """The longest K that a row count takes, and launches of eight columns each where there are more."""
     matvec_case(lb, M, 100, K, xt, "f32")
+
+
+# ------------------------------------------------------------------------------------------------ batches against the rules
+DESCENDING = [[0, 9, 2, 3], [0, 10, 2, 3, 12], [0, 2, 12, 11], [3, 0, 12], [0] + [2] * 60 + [12, 5, 12]]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("row0", DESCENDING)
+def test_append_and_read_skip_a_batch_whose_row0_descends(gpu, lb, row0):
+    """Its rows lie in several sequences, or would be counted to one that does not hold them, positions behind its own rows."""
+    s = Setup(lb, [(12, 50)], 64, 2, 16, fill=0x11, padded=2)
+    n = len(row0) - 1
+    batch = lb.Kv4Batch(torch.tensor(row0, dtype=torch.int32, device="cuda"), s.slot.repeat(n), s.pos.repeat(n), s.rows, 12, s.max_context)
+    x = torch.randn(s.rows, 2, 64, device="cuda", generator=s.gen)
+    out, err = torch.full_like(x, 9.0), torch.zeros(1, dtype=torch.int32, device="cuda")
+    s.cache().append(batch, x, x, q=x, q_out=out, rotary_dim=64, err=err)
+    assert err.item() == BAD_BATCH and (out == 9.0).all() and all((a == 0x11).all() for a in (s.k, s.ks, s.v, s.vs))
+    err.zero_()
+    s.cache().read(batch, out, None, err=err)
+    assert err.item() == BAD_BATCH and (out == 9.0).all()
