@@ -175,8 +175,8 @@ inline bool rows_vec(const ling_b200_rows& r, int type) {
 __device__ __forceinline__ size_t kv4_vector(const ling_b200_kv4& c, int page, int h, int tok) {
   return (size_t(page) * c.kv_heads + h) * c.page_tokens + tok;
 }
-// The sequence of packed row r (all lanes of a warp together, any number of sequences); -1: no sequence has it; -2: row0 descends, so
-// that it could lie in several, or be counted to one that does not hold it.
+// The sequence of packed row r (all lanes of a warp together, any number of sequences), or -1: none has it, or row0 descends, so that it
+// could lie in several, or be counted to one that does not hold it.
 __device__ __forceinline__ int kv4_find_seq(const int* __restrict__ row0, int seqs, int r) {
   int n = 0;  // sequences that end at or before r
   bool down = false;
@@ -185,8 +185,7 @@ __device__ __forceinline__ int kv4_find_seq(const int* __restrict__ row0, int se
     n += __popc(__ballot_sync(0xffffffffu, i < seqs && end <= r));
     down |= end < begin;
   }
-  if (__any_sync(0xffffffffu, down)) return -2;
-  return n < seqs && row0[n] <= r ? n : -1;
+  return !__any_sync(0xffffffffu, down) && n < seqs && row0[n] <= r ? n : -1;
 }
 struct Kv4Seq {
   int row0, n, slot, pos;

@@ -110,11 +110,16 @@ struct RowAt {
 };
 constexpr int kChunk = kThreads / 32;  // rows of a block at most
 
-// By warp: row r's place.  The error of a row whose sequence or page is out of bounds, or whose batch's row0 descends, is recorded here.
+// By one warp of a call: sequences outside the batch's bounds are recorded, whether one of the packed rows is theirs or not (one that
+// starts behind the rows has none here; where row0 descends one has fewer than none).
+__device__ __forceinline__ void record_bad_seqs(const ling_b200_kv4& c, const ling_b200_kv4_batch& b, int* err) {
+  for (int s = threadIdx.x & 31; s < b.seqs; s += 32)
+    if (!kv4_seq(c, b, s).ok) dev_fail(err, kDevBadBatch);
+}
+// By warp: row r's place.  The error of a row whose page is out of bounds is recorded here.
 __device__ __forceinline__ RowAt row_at(const ling_b200_kv4& c, const ling_b200_kv4_batch& b, int r, int* err) {
   RowAt at{0, 0, 0};
   const int s = kv4_find_seq(b.row0, b.seqs, r);
-  if (s == -2 && (threadIdx.x & 31) == 0) dev_fail(err, kDevBadBatch);
   if (s < 0) return at;  // padding behind the last sequence, or a batch against the rules
   const Kv4Seq q = kv4_seq(c, b, s);
   at.pos = q.pos + r - q.row0;
@@ -123,7 +128,7 @@ __device__ __forceinline__ RowAt row_at(const ling_b200_kv4& c, const ling_b200_
     at.rope = b.rope_pos ? b.rope_pos[r] : at.pos;
   }
   if (at.page < 1 || at.page > c.pages) {
-    if ((threadIdx.x & 31) == 0) dev_fail(err, q.ok ? int(kDevBadPage) : kDevBadBatch);
+    if ((threadIdx.x & 31) == 0 && q.ok) dev_fail(err, kDevBadPage);
     at.page = 0;
   }
   return at;
@@ -157,6 +162,7 @@ __global__ void __launch_bounds__(kThreads) kv4_append_kernel(AppendArgs a, int 
     const RowAt at = row_at(a.c, a.b, r0 + warp, a.err);
     if (lane == 0) rows[warp] = at;
   }
+  if (blockIdx.x == 0 && warp == kChunk - 1) record_bad_seqs(a.c, a.b, a.err);
   if (tid < half) freq[tid] = pow(a.theta, -2.0 * tid / a.rot);
   __syncthreads();
   for (int t = tid; t < n * half; t += kThreads) {
@@ -317,6 +323,7 @@ __global__ void __launch_bounds__(kThreads) kv4_read_kernel(ReadArgs a, int chun
     const RowAt at = row_at(a.c, a.b, r0 + warp, a.err);
     if ((tid & 31) == 0) rows[warp] = at;
   }
+  if (blockIdx.x == 0 && warp == kChunk - 1) record_bad_seqs(a.c, a.b, a.err);
   __syncthreads();
   int i = 0, left = tid;
   for (; left >= 2 * n_kv; left -= 2 * n_kv) ++i;

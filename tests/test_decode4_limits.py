@@ -4,7 +4,7 @@ import pytest
 
 torch = pytest.importorskip("torch")
 
-from test_decode4 import BAD_BATCH, Setup, matvec_case, _p  # noqa: E402
+from test_decode4 import BAD_BATCH, Setup, matvec_case, stored64, _p  # noqa: E402
 
 
 # ------------------------------------------------------------------------------------------------ refusals, without a GPU
@@ -54,3 +54,26 @@ def test_append_and_read_skip_a_batch_whose_row0_descends(gpu, lb, row0):
     err.zero_()
     s.cache().read(batch, out, None, err=err)
     assert err.item() == BAD_BATCH and (out == 9.0).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("what", ["behind the rows", "slot of none", "position of none"])
+def test_append_and_read_record_sequences_that_no_row_meets(gpu, lb, what):
+    """As the attention does: a sequence that starts behind the arrays' rows, or has no rows, and is outside the bounds."""
+    s = Setup(lb, [(5, 20), (3, 40)], 64, 1, 16, fill=0x11) if what == "behind the rows" else Setup(lb, [(5, 20), (0, 40)], 64, 1, 16, fill=0x11)
+    s.rows = 5
+    if what == "slot of none":
+        s.slot[1] = -1
+    elif what == "position of none":
+        s.pos[1] = s.max_context + 1
+    x = torch.randn(5, 1, 64, device="cuda", generator=s.gen)
+    out, q, err = torch.full_like(x, 9.0), torch.zeros(5, 2, 64, dtype=torch.bfloat16, device="cuda"), torch.zeros(1, dtype=torch.int32, device="cuda")
+    s.cache().append(s.batch(), x, x, err=err)
+    assert err.item() == BAD_BATCH
+    err.zero_()
+    s.cache().read(s.batch(), out, None, err=err)
+    assert err.item() == BAD_BATCH and torch.equal(out.double(), stored64(x.double()))
+    err.zero_()
+    work = torch.zeros(s.cache().attention_workspace_bytes(s.batch(), 2), dtype=torch.uint8, device="cuda")
+    s.cache().attention(s.batch(), q, torch.zeros_like(q), 0.1, work, err=err)
+    assert err.item() == BAD_BATCH
