@@ -228,15 +228,21 @@ __global__ void __launch_bounds__(kDecThreads, 1) kv4_decode_kernel(AttnArgs a) 
   // ---- the items' steps, end to end, and a range of them for every worker (warp 0 counts)
   if (warp == 0) {
     int sum = 0, items = 0;
+    bool down = false;
     for (int s = lane; s < a.b.seqs; s += 32) {
       const Kv4Seq q = kv4_seq(a.c, a.b, s);
       if (!q.ok && blockIdx.x == 0) dev_fail(a.err, kDevBadBatch);
+      down |= q.n < 0;
       const int mine = q.ok && q.n > 0 ? (q.n * G + kDecRows - 1) / kDecRows * H : 0;
       steps_of[s] = mine > 0 ? (q.pos + q.n + kKeys - 1) / kKeys : 0;
       first[s + 1] = mine;
       sum += mine * steps_of[s], items += mine;
     }
     sum = __reduce_add_sync(0xffffffffu, sum), items = __reduce_add_sync(0xffffffffu, items);
+    if (__any_sync(0xffffffffu, down)) {  // row0 descends: sequences may share rows, none of them is done
+      for (int s = lane; s < a.b.seqs; s += 32) first[s + 1] = 0, steps_of[s] = 0;
+      sum = items = 0;
+    }
     // no range is shorter than kMinSteps (a step for every warp of a CTA), unless the contexts themselves are
     int quota = max(max((sum + workers - 1) / workers, min(kMinSteps, sum / max(items, 1))), 1);
     const bool round = 4 * items <= workers;
@@ -792,6 +798,12 @@ __device__ __forceinline__ bool meet_all(bool ok) {
       : "memory");
   return all != 0;
 }
+// By a block: whether row0 descends somewhere, so that sequences may share rows (a barrier of its threads).
+__device__ __forceinline__ bool row0_descends(const ling_b200_kv4_batch& b) {
+  bool down = false;
+  for (int s = threadIdx.x; s < b.seqs; s += blockDim.x) down |= b.row0[s + 1] < b.row0[s];
+  return __syncthreads_or(down) != 0;
+}
 // D += A B with A in TMEM: lane = row, a column two neighbouring k.
 __device__ __forceinline__ void umma_f16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
@@ -863,7 +875,10 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv4_tile_kernel(AttnArgs a, i
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (tid < kTileMarks * 4) (&bad_keys[0][0])[tid] = 0, (&nan_keys[0][0])[tid] = 0;
-  __syncthreads();
+  if (row0_descends(a.b)) {  // (the barrier that the lines above and below need) none of the sequences is done
+    if (tid == 0 && blockIdx.x == 0 && blockIdx.y == 0 && blockIdx.z == 0) dev_fail(a.err, kDevBadBatch);
+    return;
+  }
   if (where[0] < 0) return;
   const Kv4Seq sq = kv4_seq(a.c, a.b, where[0]);
   const int f0 = where[1] * kTileRows, R = sq.n * G;  // this block's query rows f0 .. f0 + 127 of R: row f is (row f / G, head f % G)
@@ -1259,7 +1274,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv4_tile_kernel(AttnArgs a, i
 
 // The splits' partial results of the tile kernel: a warp a query row, in the order of the splits.
 template <typename T, int D>
-__global__ void __launch_bounds__(256) kv4_tile_join_kernel(AttnArgs a, int splits, int row_tiles) {
+__global__ void __launch_bounds__(256) kv4_tile_join_kernel(AttnArgs a, int splits) {
   pdl_sync();  // first statement: see common.cuh
   __shared__ int at[8];  // of the block's rows: tile * kTileRows + row of the tile; -1: none
   const int tid = threadIdx.x, lane = tid & 31, G = a.q_heads / a.c.kv_heads, H = a.c.kv_heads, h = blockIdx.y;
@@ -1288,10 +1303,9 @@ __global__ void __launch_bounds__(256) kv4_tile_join_kernel(AttnArgs a, int spli
     }
     int f = 0;
     if (seq >= 0) f = (row - a.b.row0[seq]) * G + r % G;
-    // (more tiles than rows have: sequences that share rows, against the batch's rules)
-    if (lane == 0) at[tid >> 5] = seq >= 0 && row < a.b.rows && tile0 + f / kTileRows < row_tiles ? (tile0 + f / kTileRows) * kTileRows + f % kTileRows : -1;
+    if (lane == 0) at[tid >> 5] = seq >= 0 ? (tile0 + f / kTileRows) * kTileRows + f % kTileRows : -1;
   }
-  __syncthreads();
+  if (row0_descends(a.b)) return;  // (the barrier before `at` is read)
   // ---- a thread four dims of a row: eight neighbouring rows' are 128 bytes of a partial result
   const int mine = at[tid & 7], r = blockIdx.x * 8 + (tid & 7), in = mine & (kTileRows - 1);
   if (mine < 0) return;
@@ -1405,7 +1419,7 @@ int tile_launch_t(const AttnArgs& a, const Plan& p, cudaStream_t s) {
   LB_CUDA(launch_kernel(kv4_tile_kernel<T, D>, dim3(p.row_tiles, a.c.kv_heads, p.splits), dim3(kTileThreads), size_t(TileSmem<D>::kBytes), s, a, p.splits));
   LB_LAUNCH("kv4_tile_kernel");
   if (p.splits > 1) {
-    LB_CUDA(launch_dependent(kv4_tile_join_kernel<T, D>, dim3(ceil_div(a.b.rows * (a.q_heads / a.c.kv_heads), 8), a.c.kv_heads), dim3(256), size_t(0), s, a, p.splits, p.row_tiles));
+    LB_CUDA(launch_dependent(kv4_tile_join_kernel<T, D>, dim3(ceil_div(a.b.rows * (a.q_heads / a.c.kv_heads), 8), a.c.kv_heads), dim3(256), size_t(0), s, a, p.splits));
     LB_LAUNCH("kv4_tile_join_kernel");
   }
   return LING_B200_OK;

@@ -77,3 +77,21 @@ def test_append_and_read_record_sequences_that_no_row_meets(gpu, lb, what):
     work = torch.zeros(s.cache().attention_workspace_bytes(s.batch(), 2), dtype=torch.uint8, device="cuda")
     s.cache().attention(s.batch(), q, torch.zeros_like(q), 0.1, work, err=err)
     assert err.item() == BAD_BATCH
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("G", [2, 8, 40])
+@pytest.mark.parametrize("row0", DESCENDING)
+def test_attention_skips_a_batch_whose_row0_descends(gpu, lb, row0, G):
+    """By either kernel, with split contexts and without."""
+    for pos, far in ((50, 0), (50, 1500), (3000, 0)):
+        s = Setup(lb, [(12, pos)], 64, 1, 16, fill=0x11, padded=2, slack=0)
+        n = len(row0) - 1
+        if far:  # (a bound on the context that lets the host split it)
+            s.tables, s.max_context = torch.cat([s.tables, s.tables[:, :1].repeat(1, 100)], 1), far
+        batch = lb.Kv4Batch(torch.tensor(row0, dtype=torch.int32, device="cuda"), s.slot.repeat(n), s.pos.repeat(n), s.rows, 12, s.max_context)
+        q = torch.randn(s.rows, G, 64, device="cuda", generator=s.gen).bfloat16()
+        out, lse, err = torch.full_like(q, 9.0), torch.full((s.rows, G), 9.0, device="cuda"), torch.zeros(1, dtype=torch.int32, device="cuda")
+        work = torch.full((s.cache().attention_workspace_bytes(batch, G),), 0x3f, dtype=torch.uint8, device="cuda")
+        s.cache().attention(batch, q, out, 0.125, work, lse=lse, err=err)
+        assert err.item() == BAD_BATCH and (out == 9.0).all() and (lse == 9.0).all()
