@@ -745,7 +745,8 @@ int ling_b200_kv4_append(int device, const ling_b200_kv4* cache, const ling_b200
 int ling_b200_kv4_read(int device, const ling_b200_kv4* cache, const ling_b200_kv4_batch* batch, int type, const ling_b200_rows* k,
                        const ling_b200_rows* v, int* err, void* stream);
 /* out[r][h] = softmax(scale * q[r][h] . K) V over the positions row r sees: [0, pos) of its sequence and its in-flight rows (anc, or
- * those up to itself; a call must have appended them).  q head h reads kv head h / (q_heads / kv_heads).  q (BF16 or FP16) is
+ * those up to itself; a call must have appended them).  q head h reads kv head h / (q_heads / kv_heads), rows x (q_heads / kv_heads)
+ * below 2^31 - 128.  q (BF16 or FP16) is
  * already rotated; out has its type.  lse [rows][q_heads], or NULL: log of the sum of exp(scale * q . k).  A row that sees nothing
  * has out 0 and lse -inf; NaN or infinities at positions a row does not see do not reach it.  `workspace` holds the partial
  * results of contexts that are split over SMs: as many bytes as ling_b200_kv4_attention_workspace says for the same cache

@@ -1436,10 +1436,16 @@ std::mutex g_mutex;
 
 constexpr size_t kJoinBytes = kDecMaxWorkers * sizeof(Join);
 
-bool heads_ok(const ling_b200_kv4* c, int q_heads, const char* who) {
-  if (q_heads >= 1 && q_heads <= 1024 && q_heads % c->kv_heads == 0) return true;
-  set_error(std::string(who) + ": q_heads must be a multiple of kv_heads, at most 1024");
-  return false;
+bool heads_ok(const ling_b200_kv4* c, const ling_b200_kv4_batch* b, int q_heads, const char* who) {
+  if (q_heads < 1 || q_heads > 1024 || q_heads % c->kv_heads != 0) {
+    set_error(std::string(who) + ": q_heads must be a multiple of kv_heads, at most 1024");
+    return false;
+  }
+  if ((long long)b->rows * (q_heads / c->kv_heads) > 0x7fffffffll - kTileRows) {  // (the kernels count query rows of a kv head in 32 bits)
+    set_error(std::string(who) + ": rows x (q_heads / kv_heads) is 2^31 - 128 or more");
+    return false;
+  }
+  return true;
 }
 
 }  // namespace
@@ -1450,7 +1456,7 @@ using namespace lb::d4;
 
 extern "C" size_t ling_b200_kv4_attention_workspace(const ling_b200_kv4* cache, const ling_b200_kv4_batch* batch, int q_heads) {
   const char* who = "kv4_attention_workspace";
-  if (!kv4_cache_ok(cache, who) || !kv4_batch_ok(cache, batch, who) || !heads_ok(cache, q_heads, who)) return 0;
+  if (!kv4_cache_ok(cache, who) || !kv4_batch_ok(cache, batch, who) || !heads_ok(cache, batch, q_heads, who)) return 0;
   const Plan p = make_plan(*cache, *batch, q_heads);
   if (p.tile) return kJoinBytes + (p.splits > 1 ? size_t(p.row_tiles) * cache->kv_heads * p.splits * tile_part_floats(cache->head_dim) * 4 : 0);
   return kJoinBytes + size_t(p.solo ? kDecMaxWorkers : kDecMaxCtas) * 2 * dec_part_floats(cache->head_dim) * 4;
@@ -1460,7 +1466,7 @@ extern "C" int ling_b200_kv4_attention(int device, const ling_b200_kv4* cache, c
                                        const ling_b200_rows* q, int q_heads, float scale, const ling_b200_rows* out, float* lse,
                                        void* workspace, size_t workspace_bytes, int* err, void* stream) {
   const char* who = "kv4_attention";
-  if (!kv4_cache_ok(cache, who) || !kv4_batch_ok(cache, batch, who) || !heads_ok(cache, q_heads, who)) return LING_B200_ERR_ARG;
+  if (!kv4_cache_ok(cache, who) || !kv4_batch_ok(cache, batch, who) || !heads_ok(cache, batch, q_heads, who)) return LING_B200_ERR_ARG;
   if (type != LING_B200_BF16 && type != LING_B200_F16) {
     set_error("kv4_attention: queries are LING_B200_BF16 or LING_B200_F16");
     return LING_B200_ERR_ARG;

@@ -1,10 +1,12 @@
 """Calls at the limits of the operators of a decode layer in 4 bits: sizes at which an index would leave 32 bits, batches against the
 rules, contexts so long that a sum's roundings add up, values on a rounding's border.  Refusals are checked without a GPU."""
+import ctypes as C
+
 import pytest
 
 torch = pytest.importorskip("torch")
 
-from test_decode4 import BAD_BATCH, Setup, matvec_case, stored64, _p  # noqa: E402
+from test_decode4 import BAD_BATCH, Setup, c_batch, c_cache, calls, matvec_case, stored64, _p  # noqa: E402
 
 
 # ------------------------------------------------------------------------------------------------ refusals, without a GPU
@@ -26,6 +28,15 @@ def test_matvec_refuses_activations_beyond_shared_memory(lb, K):
 def test_matvec_refuses_rows_of_weights_beyond_32_bits(lb):
     for N in ((1 << 31) - 1, (1 << 31) - 31):
         assert matvec_status(lb, 1, N, 16, lb.BF16) == lb.ERR_ARG and lb.last_error()
+
+
+@pytest.mark.parametrize("rows,G", [(1 << 24, 128), (1 << 22, 512), (1 << 21, 1024), ((1 << 24) - 1, 1024)])
+def test_attention_refuses_query_rows_beyond_32_bits(lb, rows, G):
+    """rows x heads of a group: counted in 32 bits by the kernels (an output of this size is beyond any device)."""
+    cache, batch = c_cache(lb, kv_heads=1, max_pages=1 << 20), c_batch(lb, rows=rows, max_rows=rows, max_context=rows)
+    out = (8192, G * 128, 128)
+    assert calls(lb, cache, batch, q_heads=G, q=(4096, G * 128, 128), out=out, ws=1 << 62)[2] == lb.ERR_ARG and "q_heads / kv_heads" in lb.last_error()
+    assert lb.lib().ling_b200_kv4_attention_workspace(C.byref(cache), C.byref(batch), G) == 0
 
 
 # ------------------------------------------------------------------------------------------------ products
