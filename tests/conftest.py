@@ -52,3 +52,11 @@ def gpu(lb):
     if lb.lib().ling_b200_device_count() < 1:
         pytest.skip("no CUDA device")
     return 0
+
+
+def pytest_runtest_setup(item):
+    """The refusals of the 4-bit decode operators are checked with made-up addresses, and not every call there is refused: where there
+    is a device, one that is accepted would be launched on them."""
+    if item.module.__name__.startswith("test_decode4") and "refus" in item.name and item.get_closest_marker("gpu") is None:
+        if _product().lib().ling_b200_device_count() > 0:
+            pytest.skip("made-up addresses: only without a CUDA device")
