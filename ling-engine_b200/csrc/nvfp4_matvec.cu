@@ -197,14 +197,23 @@ __global__ void __launch_bounds__(kThreads, 1) nvfp4_matvec_kernel(MatvecArgs a)
           }
         }
       }
-      // scales: a row a lane, the one or two 16-byte pieces that hold at least one of its bytes
+      // scales: a row a lane, the one or two 16-byte pieces that hold at least one of its bytes (of pieces that reach beyond the array,
+      // what lies in it)
       const int bytes = lane < rows ? min(scale_bytes - in_unit * 2, n * 2) : 0;
       const uintptr_t at = reinterpret_cast<uintptr_t>(a.scales) + size_t(row0 + (lane < rows ? lane : 0)) * scale_bytes + in_unit * 2;
       const uint8_t* w = reinterpret_cast<const uint8_t*>(at & ~uintptr_t(15));
-      cp16(st + 32 * 128 + lane * 32, w, bytes > 0 ? 16 : 0);
-      if (!scales16) {
+      const uint32_t to = st + 32 * 128 + lane * 32;
+      if (scales16) {
+        cp16(to, w, bytes > 0 ? 16 : 0);
+      } else {
+        const long long left = a.scales + size_t(a.N) * scale_bytes - w;
         const bool two = bytes > 0 && int(at & 15) + bytes > 16;
-        cp16(st + 32 * 128 + lane * 32 + 16, two ? w + 16 : w, two ? 16 : 0);
+        if (bytes > 0 && w < a.scales) {
+          for (int i = int(at & 15); i < 16 && i < left; ++i) ring[put * kStageBytes + 32 * 128 + lane * 32 + i] = w[i];
+        } else {
+          cp16(to, w, bytes > 0 ? int(min(left, 16ll)) : 0);
+        }
+        cp16(to + 16, two ? w + 16 : w, two ? int(min(left - 16, 16ll)) : 0);
       }
       put = put + 1 == S ? 0 : put + 1;
       in_unit += n;

@@ -6,7 +6,7 @@ import pytest
 
 torch = pytest.importorskip("torch")
 
-from test_decode4 import BAD_BATCH, Setup, c_batch, c_cache, calls, matvec_case, stored64, _p  # noqa: E402
+from test_decode4 import BAD_BATCH, Setup, c_batch, c_cache, calls, matvec_case, random_nvfp4, stored64, _p  # noqa: E402
 
 
 # ------------------------------------------------------------------------------------------------ refusals, without a GPU
@@ -45,6 +45,26 @@ def test_attention_refuses_query_rows_beyond_32_bits(lb, rows, G):
 def test_matvec_longest_reductions(gpu, lb, M, K, xt):
     """The longest K that a row count takes, and launches of eight columns each where there are more."""
     matvec_case(lb, M, 100, K, xt, "f32")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("N,K", [(1, 16), (5, 16), (40, 16), (33, 48), (17, 272), (75, 1088), (64, 5120), (37, 3344)])
+def test_matvec_scales_from_any_byte_on(gpu, lb, N, K):
+    """Scales inside a larger array, from every kind of byte on: as the same scales on a boundary, whatever lies around them."""
+    gen = torch.Generator("cuda").manual_seed(N + K)
+    w, ws = random_nvfp4((N, K), gen)
+    for M in (1, 9):
+        x = torch.randn(M, K, device="cuda", generator=gen).bfloat16()
+        want = torch.zeros(M, N, device="cuda")
+        lb.nvfp4_matvec(x, w, ws, 0.5, want)
+        assert torch.isfinite(want).all()
+        for off in (1, 2, 7, 15, 16):
+            around = torch.full((off + ws.numel() + 40,), 0x7f, dtype=torch.uint8, device="cuda")  # NaN
+            inside = around[off:off + ws.numel()].view(N, K // 16)
+            inside.copy_(ws)
+            got = torch.zeros(M, N, device="cuda")
+            lb.nvfp4_matvec(x, w, inside, 0.5, got)
+            assert torch.equal(got, want), (M, off)
 
 
 # ------------------------------------------------------------------------------------------------ batches against the rules
