@@ -1320,8 +1320,8 @@ __global__ void __launch_bounds__(256) kv4_tile_join_kernel(AttnArgs a, int spli
 #pragma unroll 4
   for (int s = 0; s < splits; ++s) {
     const float* p = parts + s * tile_part_floats(D);
-    const float ps = p[kTileRows * D + kTileRows + in], w = part_weight(p[kTileRows * D + in], ps, mm);
-    if (w == 0.f) continue;  // (a split without keys has written no O)
+    const float pm = p[kTileRows * D + in], ps = p[kTileRows * D + kTileRows + in], w = part_weight(pm, ps, mm);
+    if (pm == -INFINITY && ps == 0.f) continue;  // (a split without keys has written no O; one whose weight is 0 may hold a NaN)
     l = fmaf(ps, w, l);
 #pragma unroll
     for (int j = 0; j < kEach; ++j) {

@@ -1,12 +1,13 @@
 """Calls at the limits of the operators of a decode layer in 4 bits: sizes at which an index would leave 32 bits, batches against the
 rules, contexts so long that a sum's roundings add up, values on a rounding's border.  Refusals are checked without a GPU."""
 import ctypes as C
+import math
 
 import pytest
 
 torch = pytest.importorskip("torch")
 
-from test_decode4 import BAD_BATCH, Setup, c_batch, c_cache, calls, matvec_case, random_nvfp4, stored64, _p  # noqa: E402
+from test_decode4 import BAD_BATCH, Setup, T, c_batch, c_cache, calls, check_attention, e4m3_table, matvec_case, random_nvfp4, stored64, _p  # noqa: E402
 
 
 # ------------------------------------------------------------------------------------------------ refusals, without a GPU
@@ -126,3 +127,19 @@ def test_attention_skips_a_batch_whose_row0_descends(gpu, lb, row0, G):
         work = torch.full((s.cache().attention_workspace_bytes(batch, G),), 0x3f, dtype=torch.uint8, device="cuda")
         s.cache().attention(batch, q, out, 0.125, work, lse=lse, err=err)
         assert err.item() == BAD_BATCH and (out == 9.0).all() and (lse == 9.0).all()
+
+
+# ------------------------------------------------------------------------------------------------ roundings
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,G", [(1, 4), (40, 2)])
+def test_attention_nan_beside_scores_that_underflow(gpu, lb, rows, G):
+    """A row sees a NaN key (or value) whose split counts for nothing beside another split's score: NaN times 0 is NaN."""
+    for which in ("k", "v"):
+        s = Setup(lb, [(rows, 3000), (rows, 2900)], 128, 1, 16, seed=21)
+        page, tok = s.where(0, torch.tensor([2990], device="cuda"))
+        key = s.held(0, 3000)[0][2990]  # [H][D]
+        q = torch.cat([12.0 * key.float().expand(rows, G, 128), torch.randn(rows, G, 128, device="cuda", generator=s.gen)])
+        page, tok = s.where(0, torch.tensor([5], device="cuda"))
+        (s.ks if which == "k" else s.vs)[page, 0, tok] = 0x7f
+        _, out, _ = check_attention(lb, s, "bf16", G, q=q)
+        assert torch.isnan(out[:rows]).all() and torch.isfinite(out[rows:2 * rows]).all()
