@@ -3,9 +3,10 @@
 // append, of a vector x of head_dim values (a key after its rotation, a value as it is), per group g of 16 dims:
 //   s = E4M3(clamp(max |x| / 6, 2^-9, 448)),  code = the E2M1 value nearest x / s, halfway to the smaller magnitude.
 // x / s lies above a border b exactly when |x| > b * s, and b * s (3 + 4 significant bits) is exact in fp32, so the codes are
-// found by comparisons alone.  A key's rotation is carried in double and brought to fp32 by rounding to odd (the last bit set
-// when anything was cut off), which keeps every comparison with a value of fewer bits what it is for the exact number: codes
-// do not depend on how fp32 would have rounded the rotation.  Queries need no such care and turn in fp32.
+// found by comparisons alone.  A key's rotation, and its largest value over 6, are carried in double and brought to fp32 by rounding to
+// odd (the last bit set when anything was cut off), which keeps every comparison with a value of fewer bits what it is for the exact
+// number: neither codes nor scales depend on how fp32 would have rounded the rotation.  Where nothing turns, the quotient of an
+// fp32 value and 6 needs no such care: beside a middle of two E4M3 values it lies at least two thirds of an fp32 step from it.  Queries need no such care and turn in fp32.
 #include <algorithm>
 #include <cfloat>
 
@@ -220,7 +221,7 @@ __global__ void __launch_bounds__(kThreads) kv4_append_kernel(AppendArgs a, int 
             turned(j, (double(x[j]) * cs.x + o * (low ? -cs.y : cs.y)) * inv64);
           }
         }
-        amax6 = float(top / 6.0);
+        amax6 = round_to_odd(top / 6.0);  // (E4M3 keeps four bits of it: what fp32 cuts off must not make a middle of two)
       } else {
         const float inv = is_v ? v_inv : k_inv;
         float top = 0.f;

@@ -7,7 +7,7 @@ import pytest
 
 torch = pytest.importorskip("torch")
 
-from test_decode4 import BAD_BATCH, Setup, T, c_batch, c_cache, calls, check_attention, e4m3_table, matvec_case, random_nvfp4, stored64, _p  # noqa: E402
+from test_decode4 import BAD_BATCH, Setup, c_batch, c_cache, calls, check_attention, e4m3_table, matvec_case, random_nvfp4, rotated64, stored64, values64, _p  # noqa: E402
 
 
 # ------------------------------------------------------------------------------------------------ refusals, without a GPU
@@ -143,3 +143,29 @@ def test_attention_nan_beside_scores_that_underflow(gpu, lb, rows, G):
         (s.ks if which == "k" else s.vs)[page, 0, tok] = 0x7f
         _, out, _ = check_attention(lb, s, "bf16", G, q=q)
         assert torch.isnan(out[:rows]).all() and torch.isfinite(out[rows:2 * rows]).all()
+
+
+@pytest.mark.gpu
+def test_append_scales_beside_a_rounding_border(gpu, lb):
+    """Rotated keys whose largest value over 6 lies 2^-27 of itself beside the middle of two E4M3 values: the scale is the exact quotient's,
+    not that of its fp32 rounding, which is the middle itself."""
+    tab = e4m3_table()[:127]
+    lows = torch.tensor([c for c in range(0x30, 0x50)])
+    middle = (tab[lows] + tab[lows + 1]) / 2
+    want = torch.cat([middle * 6 * (1 + d) for d in (2.0 ** -27, -2.0 ** -27)])  # the group's largest value
+    n, D, p = len(want), 64, 1
+    c, sn = math.cos(p), math.sin(p)
+    x = (want / c).float()  # dims 0 and 32 turn together by p: x cos p - o sin p, o making up for what fp32 rounded off x
+    o = ((x.double() * c - want) / sn).float()
+    k = torch.full((n, 1, D), 0.125)
+    k[:, 0, 0], k[:, 0, 32] = x, o
+    turned = rotated64(k, torch.full((n,), p), D, 1e7)
+    top = turned[:, 0, :16].abs().amax(-1)
+    assert (turned[:, 0, 0].abs() == top).all() and ((top / want - 1).abs() < 2.0 ** -40).all() and torch.equal((top / 6).float().double(), torch.cat([middle, middle]))
+    k = k.cuda()
+    s = Setup(lb, [(1, p)] * n, D, 1, 16, fill=0)
+    err = torch.zeros(1, dtype=torch.int32, device="cuda")
+    s.cache().append(s.batch(), k, k, rotary_dim=D, theta=1e7, err=err)
+    page, tok = s.tables[s.slot.long(), 0].long(), p
+    got = s.ks[page, 0, tok, 0].cpu().long()
+    assert err.item() == 0 and torch.equal(got, torch.cat([lows + 1, lows]))
