@@ -13,6 +13,9 @@ namespace {
 using namespace d4;
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+// A tensor core cuts its fp32 sums off instead of rounding them, so a long chain of MMAs drifts towards 0: by 6e-9 of the sum a position,
+// measured (4e-3 over 2^19 positions).  The value product's chains end after these many positions (2.5e-5) and are added in fp32.
+constexpr int kChainKeys = 4096;
 constexpr float kPShift = 8.f;  // probabilities are carried times 2^8 in FP16: clear of its subnormals down to 2^-22
 
 struct Join;
@@ -26,6 +29,7 @@ struct AttnArgs {
   int* err;
   Join* joins;
   float* parts;
+  float* totals;  // sums of the chains that have ended (kChainKeys), where contexts are longer than one
   bool q_vec, out_vec;  // rows of q, of out start on 16-byte boundaries
 };
 
@@ -171,6 +175,8 @@ __device__ __forceinline__ float score_coef(const AttnArgs& a, float q_inv) { re
 // What a partial result (reference m, sum l) counts for under the common reference: one without a visible key has l = 0, one whose
 // scores were all NaN has l = NaN and no m.
 __device__ __forceinline__ float part_weight(float m, float l, float common) { return m == -INFINITY ? (l == 0.f ? 0.f : 1.f) : ex2(m - common); }
+// What a chain that ended under the reference `then` counts for under `now` (-inf both: no visible key yet, or NaN alone).
+__device__ __forceinline__ float chain_weight(float then, float now) { return then == now ? 1.f : ex2(then - now); }
 // B bytes of shared memory as 32-bit words.
 template <int B>
 __device__ __forceinline__ void lds(const uint8_t* p, uint32_t (&w)[B / 4]) {
@@ -434,161 +440,184 @@ __global__ void __launch_bounds__(kDecThreads, 1) kv4_decode_kernel(AttnArgs a) 
     }
 
     float o[D / 16][4] = {}, m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-    for (int n = 0; n < mine; ++n) {
-      cp_wait<S - 2>();
-      __syncwarp();  // the step has landed, for all lanes; all lanes are done with the one before, whose stage is next
-      issue();
-      const uint8_t* st = ring + stage * dec_stage_bytes(D);
-      stage = stage + 1 == S ? 0 : stage + 1;
-      const int pos0 = (step0 + turn + n * kStride) * kKeys;
-      const uint32_t ok_bits = good >> (S - 1) * U & ((1u << U) - 1u);  // block u in bit u
-      const bool masked = ok_bits != (1u << U) - 1u || pos0 + kKeys > sq.pos;
-
-      // scores
-      float s[U][4];
+    constexpr int kChain = kChainKeys / kKeys;  // steps of a chain
+    float then[2] = {-INFINITY, -INFINITY};     // reference of the chains that have ended
+    float4* totals = reinterpret_cast<float4*>(a.totals + (size_t(blockIdx.x) * kDecWarps + warp) * (kDecRows * D)) + lane;
+    auto add_totals = [&] {
+      const float w[2] = {chain_weight(then[0], m[0]), chain_weight(then[1], m[1])};
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const uint8_t* kc = st + u * dec_block_bytes(D);
-        const uint8_t* ks = kc + kK + kV;
-        float s2[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) s[u][j] = 0.f;
-#pragma unroll
-        for (int p = 0; p < KP; ++p) {
-          uint32_t w[2][KB / 4], sc[2][KB / 8];  // of keys g and g + 8: codes, scales by group as half2
-#pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            lds<KB>(kc + k_offset<D>(g, t, half, p), w[half]);
-            const uint8_t* at_s = ks + (half * 8 + g) * SB + (KB == 16 ? p * 8 + t * 2 : t);
-            const uint32_t pair = KB == 16 ? *reinterpret_cast<const uint16_t*>(at_s) : *at_s;
-            const uint32_t h = e4m3x2_to_h2(uint16_t(pair));
-            sc[half][0] = __byte_perm(h, h, 0x1010);
-            if constexpr (KB == 16) sc[half][1] = __byte_perm(h, h, 0x3232);
-          }
-#pragma unroll
-          for (int i = 0; i < KB / 4; ++i) {  // word i: 8 codes, two MMAs
-            uint32_t c[2][4];
-#pragma unroll
-            for (int half = 0; half < 2; ++half) {
-              e2m1x8_to_h2(w[half][i], c[half]);
-#pragma unroll
-              for (int j = 0; j < 4; ++j) c[half][j] = h2_mul(c[half][j], sc[half][i / 2]);
-            }
-            const int kk = p * (KB / 2) + i * 2;
-            mma_16816(s[u], c[0][0], c[1][0], c[0][1], c[1][1], qb[kk][0], qb[kk][1]);
-            mma_16816(U == 1 ? s2 : s[u], c[0][2], c[1][2], c[0][3], c[1][3], qb[kk + 1][0], qb[kk + 1][1]);  // (two chains where one block is all there is)
-          }
-        }
-        if constexpr (U == 1) {
-#pragma unroll
-          for (int j = 0; j < 4; ++j) s[u][j] += s2[j];
-        }
+      for (int i = 0; i < D / 16; ++i) {
+        const float4 x = totals[i * 32];
+        o[i][0] = fmaf(x.x, w[0], o[i][0]), o[i][1] = fmaf(x.y, w[1], o[i][1]), o[i][2] = fmaf(x.z, w[0], o[i][2]), o[i][3] = fmaf(x.w, w[1], o[i][3]);
       }
-
-      // V's scales: of this thread's key pairs (2t, 2t+1) and (2t+8, 2t+9), per group of its dims, as (key, key + 1)
-      constexpr int VG = D == 256 ? 2 : 1;
-      uint32_t vsc[U][2][VG], poison = 0;  // poison: of this thread's (block, key, row): a visible key whose V is NaN
+    };
+    for (int chain = 0; chain < mine; chain += kChain) {
+      if (chain > 0) {
+        if (chain > kChain) add_totals();
 #pragma unroll
-      for (int u = 0; u < U; ++u)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const uint8_t* at_s = st + u * dec_block_bytes(D) + kK + kV + D + (2 * t + j * 8) * SB + (D == 256 ? g * 2 : D == 128 ? g : g / 2);
-          if constexpr (D == 256) {
-            const uint32_t x = *reinterpret_cast<const uint16_t*>(at_s), y = *reinterpret_cast<const uint16_t*>(at_s + SB);
-            vsc[u][j][0] = __byte_perm(x, y, 0x0040) & 0xffffu, vsc[u][j][1] = __byte_perm(x, y, 0x0051) & 0xffffu;
-          } else {
-            vsc[u][j][0] = uint32_t(at_s[0]) | uint32_t(at_s[SB]) << 8;
-          }
+        for (int i = 0; i < D / 16; ++i) {
+          totals[i * 32] = make_float4(o[i][0], o[i][1], o[i][2], o[i][3]);
+          o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
         }
-      uint32_t vw[U][4][VB / 4];  // (asked for ahead of the softmax)
-#pragma unroll
-      for (int u = 0; u < U; ++u)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) lds<VB>(st + u * dec_block_bytes(D) + kK + v_offset<D>(g, t, j), vw[u][j]);
-      if (masked) {
-        // A V vector that is NaN must reach exactly the rows that see it: its scale is taken as 0 and its probability as NaN.
+        then[0] = m[0], then[1] = m[1];
+      }
+      const int chain_end = min(mine, chain + kChain);
+      for (int n = chain; n < chain_end; ++n) {
+        cp_wait<S - 2>();
+        __syncwarp();  // the step has landed, for all lanes; all lanes are done with the one before, whose stage is next
+        issue();
+        const uint8_t* st = ring + stage * dec_stage_bytes(D);
+        stage = stage + 1 == S ? 0 : stage + 1;
+        const int pos0 = (step0 + turn + n * kStride) * kKeys;
+        const uint32_t ok_bits = good >> (S - 1) * U & ((1u << U) - 1u);  // block u in bit u
+        const bool masked = ok_bits != (1u << U) - 1u || pos0 + kKeys > sq.pos;
+
+        // scores
+        float s[U][4];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-          uint32_t nan = 0;  // keys of this block
+          const uint8_t* kc = st + u * dec_block_bytes(D);
+          const uint8_t* ks = kc + kK + kV;
+          float s2[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int j = 0; j < 4; ++j) s[u][j] = 0.f;
+#pragma unroll
+          for (int p = 0; p < KP; ++p) {
+            uint32_t w[2][KB / 4], sc[2][KB / 8];  // of keys g and g + 8: codes, scales by group as half2
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+              lds<KB>(kc + k_offset<D>(g, t, half, p), w[half]);
+              const uint8_t* at_s = ks + (half * 8 + g) * SB + (KB == 16 ? p * 8 + t * 2 : t);
+              const uint32_t pair = KB == 16 ? *reinterpret_cast<const uint16_t*>(at_s) : *at_s;
+              const uint32_t h = e4m3x2_to_h2(uint16_t(pair));
+              sc[half][0] = __byte_perm(h, h, 0x1010);
+              if constexpr (KB == 16) sc[half][1] = __byte_perm(h, h, 0x3232);
+            }
+#pragma unroll
+            for (int i = 0; i < KB / 4; ++i) {  // word i: 8 codes, two MMAs
+              uint32_t c[2][4];
+#pragma unroll
+              for (int half = 0; half < 2; ++half) {
+                e2m1x8_to_h2(w[half][i], c[half]);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) c[half][j] = h2_mul(c[half][j], sc[half][i / 2]);
+              }
+              const int kk = p * (KB / 2) + i * 2;
+              mma_16816(s[u], c[0][0], c[1][0], c[0][1], c[1][1], qb[kk][0], qb[kk][1]);
+              mma_16816(U == 1 ? s2 : s[u], c[0][2], c[1][2], c[0][3], c[1][3], qb[kk + 1][0], qb[kk + 1][1]);  // (two chains where one block is all there is)
+            }
+          }
+          if constexpr (U == 1) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) s[u][j] += s2[j];
+          }
+        }
+
+        // V's scales: of this thread's key pairs (2t, 2t+1) and (2t+8, 2t+9), per group of its dims, as (key, key + 1)
+        constexpr int VG = D == 256 ? 2 : 1;
+        uint32_t vsc[U][2][VG], poison = 0;  // poison: of this thread's (block, key, row): a visible key whose V is NaN
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const uint8_t* at_s = st + u * dec_block_bytes(D) + kK + kV + D + (2 * t + j * 8) * SB + (D == 256 ? g * 2 : D == 128 ? g : g / 2);
+            if constexpr (D == 256) {
+              const uint32_t x = *reinterpret_cast<const uint16_t*>(at_s), y = *reinterpret_cast<const uint16_t*>(at_s + SB);
+              vsc[u][j][0] = __byte_perm(x, y, 0x0040) & 0xffffu, vsc[u][j][1] = __byte_perm(x, y, 0x0051) & 0xffffu;
+            } else {
+              vsc[u][j][0] = uint32_t(at_s[0]) | uint32_t(at_s[SB]) << 8;
+            }
+          }
+        uint32_t vw[U][4][VB / 4];  // (asked for ahead of the softmax)
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) lds<VB>(st + u * dec_block_bytes(D) + kK + v_offset<D>(g, t, j), vw[u][j]);
+        if (masked) {
+          // A V vector that is NaN must reach exactly the rows that see it: its scale is taken as 0 and its probability as NaN.
+#pragma unroll
+          for (int u = 0; u < U; ++u) {
+            uint32_t nan = 0;  // keys of this block
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+              for (int v = 0; v < VG; ++v)
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+                  if ((vsc[u][j][v] >> (8 * e) & 0x7fu) == 0x7fu) {
+                    nan |= 1u << (2 * t + j * 8 + e);
+                    vsc[u][j][v] &= e ? 0x00ffu : 0xff00u;
+                  }
+            nan = __reduce_or_sync(0xffffffffu, nan);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const int key = g + (j >> 1) * 8, pos = pos0 + u * 16 + key, i = pos - sq.pos;
+              const uint32_t mask = see[j & 1];
+              const bool visible = (ok_bits >> u & 1u) && pos < keys && (i < 0 || (a.b.anc ? (mask >> i & 1u) : i < int(mask)));
+              if (!visible) s[u][j] = -INFINITY;
+              else poison |= (nan >> key & 1u) << (u * 4 + j);
+            }
+          }
+        }
+
+        // Scores are s * coef, coef >= 0.  The sums are kept relative to a reference m of each row, not its maximum: as long as no score exceeds it by 2^kLazy,
+        // P (times 2^8) stays inside FP16 and nothing is exchanged or scaled.  Rows are columns 2t, 2t + 1; keys lie across the
+        // lanes with the same t.
+        float mx[2] = {fmaxf(s[0][0], s[0][2]), fmaxf(s[0][1], s[0][3])};
+#pragma unroll
+        for (int u = 1; u < U; ++u) mx[0] = fmaxf(mx[0], fmaxf(s[u][0], s[u][2])), mx[1] = fmaxf(mx[1], fmaxf(s[u][1], s[u][3]));
+        if (__any_sync(0xffffffffu, fmaf(mx[0], coef[0], -m[0]) > kLazy || fmaf(mx[1], coef[1], -m[1]) > kLazy)) {
+          float keep[2];
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+#pragma unroll
+            for (int x = 4; x < 32; x <<= 1) mx[j] = fmaxf(mx[j], __shfl_xor_sync(0xffffffffu, mx[j], x));
+            mx[j] = fmaxf(mx[j] * coef[j], m[j]);
+            keep[j] = m[j] == -INFINITY ? 0.f : ex2(m[j] - mx[j]);
+            l[j] *= keep[j];
+            m[j] = mx[j];
+          }
+#pragma unroll
+          for (int i = 0; i < D / 16; ++i) o[i][0] *= keep[0], o[i][2] *= keep[0], o[i][1] *= keep[1], o[i][3] *= keep[1];
+        }
+        const float base[2] = {m[0] == -INFINITY ? 0.f : m[0] - kPShift, m[1] == -INFINITY ? 0.f : m[1] - kPShift};
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          float p[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) p[j] = ex2(fmaf(s[u][j], coef[j & 1], -base[j & 1]));
+          l[0] += p[0] + p[2], l[1] += p[1] + p[3];
+          if (poison) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) p[j] = poison >> (u * 4 + j) & 1u ? NAN : p[j];
+          }
+          const uint32_t b0 = movmatrix(h2(p[0], p[1])), b1 = movmatrix(h2(p[2], p[3]));
+          uint32_t vh[2][VG];
 #pragma unroll
           for (int j = 0; j < 2; ++j)
 #pragma unroll
-            for (int v = 0; v < VG; ++v)
+            for (int x = 0; x < VG; ++x) vh[j][x] = e4m3x2_to_h2(uint16_t(vsc[u][j][x]));
 #pragma unroll
-              for (int e = 0; e < 2; ++e)
-                if ((vsc[u][j][v] >> (8 * e) & 0x7fu) == 0x7fu) {
-                  nan |= 1u << (2 * t + j * 8 + e);
-                  vsc[u][j][v] &= e ? 0x00ffu : 0xff00u;
-                }
-          nan = __reduce_or_sync(0xffffffffu, nan);
+          for (int i = 0; i < VB / 4; ++i) {  // word i: 8 dims, four MMAs' rows g (even dims) and g + 8 (odd dims)
+            uint32_t even[2][4], odd[2][4];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int key = g + (j >> 1) * 8, pos = pos0 + u * 16 + key, i = pos - sq.pos;
-            const uint32_t mask = see[j & 1];
-            const bool visible = (ok_bits >> u & 1u) && pos < keys && (i < 0 || (a.b.anc ? (mask >> i & 1u) : i < int(mask)));
-            if (!visible) s[u][j] = -INFINITY;
-            else poison |= (nan >> key & 1u) << (u * 4 + j);
-          }
-        }
-      }
-
-      // Scores are s * coef, coef >= 0.  The sums are kept relative to a reference m of each row, not its maximum: as long as no score exceeds it by 2^kLazy,
-      // P (times 2^8) stays inside FP16 and nothing is exchanged or scaled.  Rows are columns 2t, 2t + 1; keys lie across the
-      // lanes with the same t.
-      float mx[2] = {fmaxf(s[0][0], s[0][2]), fmaxf(s[0][1], s[0][3])};
+            for (int j = 0; j < 2; ++j) {
+              const uint32_t x = vw[u][2 * j][i], y = vw[u][2 * j + 1][i];
+              e2m1x8_to_h2(x & 0x0f0f0f0fu | (y << 4 & 0xf0f0f0f0u), even[j]);
+              e2m1x8_to_h2(x >> 4 & 0x0f0f0f0fu | y & 0xf0f0f0f0u, odd[j]);
 #pragma unroll
-      for (int u = 1; u < U; ++u) mx[0] = fmaxf(mx[0], fmaxf(s[u][0], s[u][2])), mx[1] = fmaxf(mx[1], fmaxf(s[u][1], s[u][3]));
-      if (__any_sync(0xffffffffu, fmaf(mx[0], coef[0], -m[0]) > kLazy || fmaf(mx[1], coef[1], -m[1]) > kLazy)) {
-        float keep[2];
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-#pragma unroll
-          for (int x = 4; x < 32; x <<= 1) mx[j] = fmaxf(mx[j], __shfl_xor_sync(0xffffffffu, mx[j], x));
-          mx[j] = fmaxf(mx[j] * coef[j], m[j]);
-          keep[j] = m[j] == -INFINITY ? 0.f : ex2(m[j] - mx[j]);
-          l[j] *= keep[j];
-          m[j] = mx[j];
-        }
-#pragma unroll
-        for (int i = 0; i < D / 16; ++i) o[i][0] *= keep[0], o[i][2] *= keep[0], o[i][1] *= keep[1], o[i][3] *= keep[1];
-      }
-      const float base[2] = {m[0] == -INFINITY ? 0.f : m[0] - kPShift, m[1] == -INFINITY ? 0.f : m[1] - kPShift};
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        float p[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) p[j] = ex2(fmaf(s[u][j], coef[j & 1], -base[j & 1]));
-        l[0] += p[0] + p[2], l[1] += p[1] + p[3];
-        if (poison) {
-#pragma unroll
-          for (int j = 0; j < 4; ++j) p[j] = poison >> (u * 4 + j) & 1u ? NAN : p[j];
-        }
-        const uint32_t b0 = movmatrix(h2(p[0], p[1])), b1 = movmatrix(h2(p[2], p[3]));
-        uint32_t vh[2][VG];
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-          for (int x = 0; x < VG; ++x) vh[j][x] = e4m3x2_to_h2(uint16_t(vsc[u][j][x]));
-#pragma unroll
-        for (int i = 0; i < VB / 4; ++i) {  // word i: 8 dims, four MMAs' rows g (even dims) and g + 8 (odd dims)
-          uint32_t even[2][4], odd[2][4];
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const uint32_t x = vw[u][2 * j][i], y = vw[u][2 * j + 1][i];
-            e2m1x8_to_h2(x & 0x0f0f0f0fu | (y << 4 & 0xf0f0f0f0u), even[j]);
-            e2m1x8_to_h2(x >> 4 & 0x0f0f0f0fu | y & 0xf0f0f0f0u, odd[j]);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const uint32_t f = vh[j][VG == 2 ? i / 2 : 0];
-              even[j][e] = h2_mul(even[j][e], f), odd[j][e] = h2_mul(odd[j][e], f);
+              for (int e = 0; e < 4; ++e) {
+                const uint32_t f = vh[j][VG == 2 ? i / 2 : 0];
+                even[j][e] = h2_mul(even[j][e], f), odd[j][e] = h2_mul(odd[j][e], f);
+              }
             }
-          }
 #pragma unroll
-          for (int e = 0; e < 4; ++e) mma_16816(o[i * 4 + e], even[0][e], odd[0][e], even[1][e], odd[1][e], b0, b1);
+            for (int e = 0; e < 4; ++e) mma_16816(o[i * 4 + e], even[0][e], odd[0][e], even[1][e], odd[1][e], b0, b1);
+          }
         }
       }
     }
-
+    if (mine > kChain) add_totals();
 #pragma unroll
     for (int j = 0; j < 2; ++j)
 #pragma unroll
@@ -1435,6 +1464,15 @@ DeviceInfo g_devices[kMaxDevices];
 std::mutex g_mutex;
 
 constexpr size_t kJoinBytes = kDecMaxWorkers * sizeof(Join);
+// Floats of partial results, and of the totals of ended chains behind them.
+size_t part_floats(const Plan& p, const ling_b200_kv4& c) {
+  if (p.tile) return p.splits > 1 ? size_t(p.row_tiles) * c.kv_heads * p.splits * tile_part_floats(c.head_dim) : 0;
+  return size_t(p.solo ? kDecMaxWorkers : kDecMaxCtas) * 2 * dec_part_floats(c.head_dim);
+}
+size_t total_floats(const Plan& p, const ling_b200_kv4& c, const ling_b200_kv4_batch& b) {
+  if (p.tile) return 0;
+  return b.max_context > (p.solo ? 1 : kDecWarps) * kChainKeys ? size_t(kDecMaxCtas) * kDecWarps * kDecRows * c.head_dim : 0;  // (a warp's longest share)
+}
 
 bool heads_ok(const ling_b200_kv4* c, const ling_b200_kv4_batch* b, int q_heads, const char* who) {
   if (q_heads < 1 || q_heads > 1024 || q_heads % c->kv_heads != 0) {
@@ -1458,8 +1496,7 @@ extern "C" size_t ling_b200_kv4_attention_workspace(const ling_b200_kv4* cache, 
   const char* who = "kv4_attention_workspace";
   if (!kv4_cache_ok(cache, who) || !kv4_batch_ok(cache, batch, who) || !heads_ok(cache, batch, q_heads, who)) return 0;
   const Plan p = make_plan(*cache, *batch, q_heads);
-  if (p.tile) return kJoinBytes + (p.splits > 1 ? size_t(p.row_tiles) * cache->kv_heads * p.splits * tile_part_floats(cache->head_dim) * 4 : 0);
-  return kJoinBytes + size_t(p.solo ? kDecMaxWorkers : kDecMaxCtas) * 2 * dec_part_floats(cache->head_dim) * 4;
+  return kJoinBytes + (part_floats(p, *cache) + total_floats(p, *cache, *batch)) * 4;
 }
 
 extern "C" int ling_b200_kv4_attention(int device, const ling_b200_kv4* cache, const ling_b200_kv4_batch* batch, int type,
@@ -1493,7 +1530,8 @@ extern "C" int ling_b200_kv4_attention(int device, const ling_b200_kv4* cache, c
   int sms = 0;
   if (const int r = enter_device(guard, device, g_devices, g_mutex, attention_init, &sms)) return r;
   AttnArgs a{*cache, *batch, *q, *out, q_heads, scale, lse, err, static_cast<Join*>(workspace),
-             reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + kJoinBytes), rows_vec(*q, type), rows_vec(*out, type)};
+             reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + kJoinBytes), nullptr, rows_vec(*q, type), rows_vec(*out, type)};
+  a.totals = a.parts + part_floats(make_plan(*cache, *batch, q_heads), *cache);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   return type == LING_B200_BF16 ? attention_launch<__nv_bfloat16>(a, sms, s) : attention_launch<__half>(a, sms, s);
 }

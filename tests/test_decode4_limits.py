@@ -145,6 +145,43 @@ def test_attention_nan_beside_scores_that_underflow(gpu, lb, rows, G):
         assert torch.isnan(out[:rows]).all() and torch.isfinite(out[rows:2 * rows]).all()
 
 
+def constant_values(lb, kind, D, n):
+    """Attention over n positions whose V is one vector: (output, that vector).  Each probability is off by half an FP16 step at most."""
+    seqs, rows, G = {"warps alone": (1024, 1, 16), "warps together": (73, 1, 4), "tiles": (1, 1200, 16)}[kind]
+    page, gen = 64, torch.Generator("cuda").manual_seed(n + D)
+    pages = -(-(n + rows) // page)
+    k = torch.randint(0, 256, (pages + 1, 1, page, D // 2), dtype=torch.uint8, device="cuda", generator=gen)
+    ks = torch.full((pages + 1, 1, page, D // 16), 0x30, dtype=torch.uint8, device="cuda")  # 1/2
+    v_one = torch.randint(0, 256, (D // 2,), dtype=torch.uint8, device="cuda", generator=gen)
+    vs_one = (0x38 + torch.arange(D // 16, device="cuda") % 8).to(torch.uint8)
+    v, vs = v_one.expand(pages + 1, 1, page, D // 2).contiguous(), vs_one.expand(pages + 1, 1, page, D // 16).contiguous()
+    tables = torch.arange(1, pages + 1, dtype=torch.int32, device="cuda").view(1, -1)
+    cache = lb.Kv4Cache(k, ks, v, vs, tables)
+    full = lambda x: torch.full((seqs,), x, dtype=torch.int32, device="cuda")
+    batch = lb.Kv4Batch(torch.arange(seqs + 1, dtype=torch.int32, device="cuda") * rows, full(0), full(n), seqs * rows, rows, n + rows)
+    q = torch.randn(seqs * rows, G, D, device="cuda", generator=gen).half()
+    out, err = torch.zeros_like(q), torch.zeros(1, dtype=torch.int32, device="cuda")
+    work = torch.empty(cache.attention_workspace_bytes(batch, G), dtype=torch.uint8, device="cuda")
+    cache.attention(batch, q, out, 1 / math.sqrt(D), work, err=err)
+    assert err.item() == 0
+    return out.double(), values64(v_one, vs_one)
+
+
+def check_constant_values(lb, kind, D, n):
+    """out = V.  Half an FP16 step each for the output and the probabilities, and what a chain of tensor-core sums loses: at most 2^-23 of
+    the sum a link of 16 positions, which must not go on over the whole context (at n = 2^20 that would be up to 2^-7): 2^-14 for 512 links."""
+    out, v = constant_values(lb, kind, D, n)
+    off = ((out - v).abs() / v.abs().clamp(min=2.0 ** -10)).max().item()
+    assert off <= 2.0 ** -11 + 2.0 ** -11 + 2.0 ** -14, off
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["warps alone", "warps together"])
+@pytest.mark.parametrize("D,n", [(64, 1 << 20), (128, 300001), (256, 1 << 19), (256, 4097), (64, 4095)])
+def test_attention_sums_over_long_contexts_of_a_warp(gpu, lb, kind, D, n):
+    check_constant_values(lb, kind, D, n)
+
+
 @pytest.mark.gpu
 def test_append_scales_beside_a_rounding_border(gpu, lb):
     """Rotated keys whose largest value over 6 lies 2^-27 of itself beside the middle of two E4M3 values: the scale is the exact quotient's,
