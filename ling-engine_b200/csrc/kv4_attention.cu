@@ -14,8 +14,9 @@ using namespace d4;
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 // A tensor core cuts its fp32 sums off instead of rounding them, so a long chain of MMAs drifts towards 0: by 6e-9 of the sum a position,
-// measured (4e-3 over 2^19 positions).  The value product's chains end after these many positions (2.5e-5) and are added in fp32.
-constexpr int kChainKeys = 4096;
+// measured (4e-3 over 2^19 positions).  The value product's chains end after these many positions (2.5e-5, in the tile kernel, which
+// waits for its MMAs there, 5e-5) and are added in fp32.
+constexpr int kChainKeys = 4096, kTileChainKeys = 8192;
 constexpr float kPShift = 8.f;  // probabilities are carried times 2^8 in FP16: clear of its subnormals down to 2^-22
 
 struct Join;
@@ -798,7 +799,7 @@ __global__ void __launch_bounds__(kJoinThreads) kv4_join_kernel(AttnArgs a) {
 // without warps of their own for each, was slower (840 and 909 us): more overlap only meets at shared memory.
 // Every wait is bounded; one that runs out is recorded and the CTA leaves with its TMEM freed.
 constexpr int kTileRows = 128, kTileKeys = 128, kTileWarps = 17, kTileThreads = kTileWarps * 32, kTileWorkers = 256, kTileMarks = 8;
-constexpr int kMmaWarp = 16;
+constexpr int kMmaWarp = 16, kTileChain = kTileChainKeys / kTileKeys;  // tiles of a chain of value products
 template <int D>
 struct TileSmem {
   static constexpr int kOperand = 256 * D;  // 128 rows of D halves: [D / 64][128][128 B]
@@ -916,7 +917,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv4_tile_kernel(AttnArgs a, i
   const int all_see = a.b.anc ? sq.pos : sq.pos + f0 / G + 1;                     // every row sees at least these
   const int tiles = (keys + kTileKeys - 1) / kTileKeys;
   const int t0 = int((long long)tiles * blockIdx.z / splits), nt = int((long long)tiles * (blockIdx.z + 1) / splits) - t0;
-  auto partial = [&] { return a.parts + ((size_t(index) * H + h) * splits + blockIdx.z) * tile_part_floats(D); };
+  auto partial = [&] { return a.parts + ((size_t(index) * H + h) * splits + blockIdx.z) * tile_part_floats(D); };  // (splits > 1, or nt > kTileChain)
   if (nt == 0) {  // (more splits than tiles)
     if (tid < kTileRows) partial()[kTileRows * D + tid] = -INFINITY, partial()[kTileRows * D + kTileRows + tid] = 0.f;
     return;
@@ -1010,7 +1011,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv4_tile_kernel(AttnArgs a, i
 #pragma unroll
         for (int k = 0; k < kTileKeys / 16; ++k)
           umma_f16_ts(tmem + kOcol, tmem + uint32_t(t & 1) * kTileKeys + uint32_t((k >> 2) * 64 + (k & 3) * 8),
-                      desc_mn_sw128(smem_u32(vs + k * 16 * 128), kTileKeys * 128), kIdescO, (t | k) ? 1u : 0u);
+                      desc_mn_sw128(smem_u32(vs + k * 16 * 128), kTileKeys * 128), kIdescO, (t % kTileChain | k) ? 1u : 0u);
         umma_commit(&pv_done[t & 1]);
       }
     }
@@ -1135,7 +1136,17 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv4_tile_kernel(AttnArgs a, i
     const uint32_t see = real && a.b.anc ? a.b.anc[sq.row0 + i_row] : 0u;
     const int limit = real ? sq.pos + i_row + 1 : 0;  // (no masks) positions this row sees
     const uint32_t lane_addr = tmem + (uint32_t((warp & 3) * 32) << 16);
-    float m = -INFINITY, l = 0.f;
+    float m = -INFINITY, l = 0.f, then = -INFINITY;  // then: reference of the chains that have ended
+    // 32 dims (from 32 c on) of this row's total of the ended chains, where its partial result will lie, times w, added to x
+    auto add_total = [&](int c, float w, uint32_t (&x)[32]) {
+      const float* total = partial();
+#pragma unroll
+      for (int j = 0; j < 32; j += 4) {
+        const float4 y = *reinterpret_cast<const float4*>(total + (size_t(c * 8 + j / 4) * kTileRows + r) * 4);
+        x[j] = __float_as_uint(fmaf(y.x, w, __uint_as_float(x[j]))), x[j + 1] = __float_as_uint(fmaf(y.y, w, __uint_as_float(x[j + 1])));
+        x[j + 2] = __float_as_uint(fmaf(y.z, w, __uint_as_float(x[j + 2]))), x[j + 3] = __float_as_uint(fmaf(y.w, w, __uint_as_float(x[j + 3])));
+      }
+    };
     bool ok = true;
     for (int t = 0; t < nt; ++t) {
       ok = ok && wait(&qk_done[t & 1], t >> 1, kDevWaitTmemFull);
@@ -1182,12 +1193,29 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv4_tile_kernel(AttnArgs a, i
       if (!ok) break;
       mx = fmaxf(mx, row_max[t & 1][half ^ 1][r]);
       if (masked) ok = (t == 0 || wait(&pv_done[(t - 1) & 1], (t - 1) >> 1, kDevWaitTmemFull)) && wait(&v_full, t, kDevWaitFull);  // the marks of V's NaN
+      if (t % kTileChain == 0 && t > 0) {  // a chain ends
+        ok = ok && wait(&pv_done[(t - 1) & 1], (t - 1) >> 1, kDevWaitTmemFull);  // O is complete
+        tc_fence_after();
+        const float w = chain_weight(then, m);
+#pragma unroll 1
+        for (int c = half * (D / 64); c < (half + 1) * (D / 64); ++c) {
+          uint32_t x[32];
+          tmem_ld32(lane_addr + kOcol + c * 32, x);
+          tmem_ld_wait();
+          if (t > kTileChain) add_total(c, w, x);
+          float* total = partial();
+#pragma unroll
+          for (int j = 0; j < 32; j += 4)
+            *reinterpret_cast<uint4*>(total + (size_t(c * 8 + j / 4) * kTileRows + r) * 4) = make_uint4(x[j], x[j + 1], x[j + 2], x[j + 3]);
+        }
+        then = m;
+      }
       const float top = mx * coef;  // (-inf where nothing is seen)
       const bool grow = top > m + kLazy;
       if (__any_sync(0xffffffffu, grow)) {
         const float m_new = grow ? top : m, keep = m == -INFINITY ? 0.f : ex2(m - m_new);
         l *= keep, m = m_new;
-        if (t > 0) {
+        if (t % kTileChain != 0) {  // (where a chain starts, O is written anew)
           ok = ok && wait(&pv_done[(t - 1) & 1], (t - 1) >> 1, kDevWaitTmemFull);  // O is complete
           tc_fence_after();
 #pragma unroll 1
@@ -1259,6 +1287,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv4_tile_kernel(AttnArgs a, i
         uint32_t x[32];
         tmem_ld32(lane_addr + kOcol + c * 32, x);
         tmem_ld_wait();
+        if (nt > kTileChain) add_total(c, chain_weight(then, m), x);
         if (splits > 1) {  // [dims / 4][row][4]
 #pragma unroll
           for (int j = 0; j < 32; j += 4)
@@ -1464,9 +1493,10 @@ DeviceInfo g_devices[kMaxDevices];
 std::mutex g_mutex;
 
 constexpr size_t kJoinBytes = kDecMaxWorkers * sizeof(Join);
-// Floats of partial results, and of the totals of ended chains behind them.
-size_t part_floats(const Plan& p, const ling_b200_kv4& c) {
-  if (p.tile) return p.splits > 1 ? size_t(p.row_tiles) * c.kv_heads * p.splits * tile_part_floats(c.head_dim) : 0;
+// Floats of partial results (the tile kernel's ended chains are added up in their place), and of the totals of the decode kernel's ended
+// chains behind them.
+size_t part_floats(const Plan& p, const ling_b200_kv4& c, const ling_b200_kv4_batch& b) {
+  if (p.tile) return p.splits > 1 || b.max_context > kTileChainKeys ? size_t(p.row_tiles) * c.kv_heads * p.splits * tile_part_floats(c.head_dim) : 0;
   return size_t(p.solo ? kDecMaxWorkers : kDecMaxCtas) * 2 * dec_part_floats(c.head_dim);
 }
 size_t total_floats(const Plan& p, const ling_b200_kv4& c, const ling_b200_kv4_batch& b) {
@@ -1496,7 +1526,7 @@ extern "C" size_t ling_b200_kv4_attention_workspace(const ling_b200_kv4* cache, 
   const char* who = "kv4_attention_workspace";
   if (!kv4_cache_ok(cache, who) || !kv4_batch_ok(cache, batch, who) || !heads_ok(cache, batch, q_heads, who)) return 0;
   const Plan p = make_plan(*cache, *batch, q_heads);
-  return kJoinBytes + (part_floats(p, *cache) + total_floats(p, *cache, *batch)) * 4;
+  return kJoinBytes + (part_floats(p, *cache, *batch) + total_floats(p, *cache, *batch)) * 4;
 }
 
 extern "C" int ling_b200_kv4_attention(int device, const ling_b200_kv4* cache, const ling_b200_kv4_batch* batch, int type,
@@ -1531,7 +1561,7 @@ extern "C" int ling_b200_kv4_attention(int device, const ling_b200_kv4* cache, c
   if (const int r = enter_device(guard, device, g_devices, g_mutex, attention_init, &sms)) return r;
   AttnArgs a{*cache, *batch, *q, *out, q_heads, scale, lse, err, static_cast<Join*>(workspace),
              reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + kJoinBytes), nullptr, rows_vec(*q, type), rows_vec(*out, type)};
-  a.totals = a.parts + part_floats(make_plan(*cache, *batch, q_heads), *cache);
+  a.totals = a.parts + part_floats(make_plan(*cache, *batch, q_heads), *cache, *batch);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   return type == LING_B200_BF16 ? attention_launch<__nv_bfloat16>(a, sms, s) : attention_launch<__half>(a, sms, s);
 }

@@ -183,6 +183,12 @@ def test_attention_sums_over_long_contexts_of_a_warp(gpu, lb, kind, D, n):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("D,n", [(64, 1 << 20), (128, 300001), (256, 1 << 19), (256, 8193), (64, 8192 - 1200)])
+def test_attention_sums_over_long_contexts_of_a_tile(gpu, lb, D, n):
+    check_constant_values(lb, "tiles", D, n)
+
+
+@pytest.mark.gpu
 def test_append_scales_beside_a_rounding_border(gpu, lb):
     """Rotated keys whose largest value over 6 lies 2^-27 of itself beside the middle of two E4M3 values: the scale is the exact quotient's,
     not that of its fp32 rounding, which is the middle itself."""
@@ -206,3 +212,19 @@ def test_append_scales_beside_a_rounding_border(gpu, lb):
     page, tok = s.tables[s.slot.long(), 0].long(), p
     got = s.ks[page, 0, tok, 0].cpu().long()
     assert err.item() == 0 and torch.equal(got, torch.cat([lows + 1, lows]))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("seqs,G", [([(600, 20000), (600, 17000)], 8), ([(1, 50000 - 100 * i) for i in range(100)], 24)])
+def test_attention_scores_that_grow_from_chain_to_chain(gpu, lb, seqs, G):
+    """Keys whose size grows along the context, so that the reference moves after a chain has ended; a NaN value in the last sequence's
+    first chain."""
+    s = Setup(lb, seqs, 64, 1, 64, seed=23)
+    for i, (r, p) in enumerate(seqs):
+        n = -(-(r + p) // 64)
+        s.ks[s.tables[s.slot[i].long(), :n].long()] = (0x10 + 40 * torch.arange(n, device="cuda") // n).to(torch.uint8)[:, None, None, None]
+    page, tok = s.where(len(seqs) - 1, torch.tensor([5], device="cuda"))
+    s.vs[page, 0, tok] = 0x7f
+    _, out, _ = check_attention(lb, s, "bf16", G, spread=2.0, lse=False)
+    last = seqs[-1][0]
+    assert torch.isnan(out[-last:]).all() and torch.isfinite(out[:-last]).all()
