@@ -695,8 +695,8 @@ enum { LING_B200_F32 = 0, LING_B200_BF16 = 1, LING_B200_F16 = 2 }; /* element ty
 /* y[m][n] = alpha * sum_k x[m][k] * w[n][k] (or += with accumulate) for M rows, 1 <= M <= 32; w as ling_b200_quantize_nvfp4_host leaves it
  * (values [N][K/2], scales [N][K/16], K % 16 == 0; alpha carries the tensor scale).  x [M][ldx], y [M][ldy] of any two of the
  * types above, ldx >= K, ldy >= N in elements; y must not overlap x.  x stays in its type (fp32 included: no activation
- * quantizer, unlike ling_b200_prefill_gemm_nvfp4_host), sums are fp32, each y is rounded once.  A row's result does
- * not depend on what the other rows hold.  values on an 8-byte boundary.  N up to 2^31 - 32;
+ * quantizer, unlike ling_b200_prefill_gemm_nvfp4_host; a BF16 or fp32 element counts to within 2^-39 of its row's largest, fp32 to
+ * within 2^-23 of itself besides), sums are fp32, each y is rounded once.  A row's result does not depend on what the other rows hold.  values on an 8-byte boundary.  N up to 2^31 - 32;
  * K up to 57344 (up to four 16-bit or two fp32 rows: 114688, one 16-bit row: 462848); ERR_UNSUPPORTED where the activations of eight columns
  * (a 16-bit row is one, an fp32 row two), or of as many as there are, no longer fit a cluster's shared memory. */
 int ling_b200_nvfp4_matvec(int device, const void* x, int x_type, long long ldx, int M, const uint8_t* values, const uint8_t* scales,
@@ -746,7 +746,7 @@ int ling_b200_kv4_read(int device, const ling_b200_kv4* cache, const ling_b200_k
                        const ling_b200_rows* v, int* err, void* stream);
 /* out[r][h] = softmax(scale * q[r][h] . K) V over the positions row r sees: [0, pos) of its sequence and its in-flight rows (anc, or
  * those up to itself; a call must have appended them).  q head h reads kv head h / (q_heads / kv_heads), rows x (q_heads / kv_heads)
- * below 2^31 - 128.  q (BF16 or FP16) is
+ * below 2^31 - 128.  q (BF16 or FP16; an element counts to within 2^-33 of the largest of its row and head) is
  * already rotated; out has its type.  lse [rows][q_heads], or NULL: log of the sum of exp(scale * q . k).  A row that sees nothing
  * has out 0 and lse -inf; NaN or infinities at positions a row does not see do not reach it.  `workspace` holds the partial
  * results of contexts that are split over SMs: as many bytes as ling_b200_kv4_attention_workspace says for the same cache

@@ -42,7 +42,8 @@ struct AttnArgs {
 //                 key's 4 neighbouring codes per MMA (the order of dims is free as long as Q's fragments follow it), for O^T
 //                 the same byte of two neighbouring keys, nibbles merged so that one cvt gives (key, key + 1) of a dim.  P
 //                 turns from an accumulator into a B fragment by movmatrix.  Values in FP16 are exact (E2M1 x E4M3 has 6
-//                 significant bits); q goes to FP16 times a power of two of its row, which loses nothing that a sum in fp32 keeps.
+//                 significant bits); q goes to FP16 times a power of two of its row: an element is off by at most 2^-33 of the
+//                 row's largest, under what a sum in fp32 keeps as long as the largest meet keys that are not 0.
 //   loads         every warp streams its own steps (4.5 KB: 16, 32 or 64 keys) by cp.async through a private ring; the ring runs
 //                 on across the items of a CTA, and nothing inside an item waits for another warp.
 //   balance       the steps of all (sequence, kv head, row tile) items lie end to end and are cut into equal ranges, one per

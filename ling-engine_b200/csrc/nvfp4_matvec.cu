@@ -8,9 +8,10 @@
 //                 row (16 bytes, two scales), four to an MMA; the order of k is free as long as the activations follow it.  A
 //                 weight is exact in FP16 (E2M1 x E4M3 has 6 significant bits).
 //   activations   FP16 as they are; BF16 and fp32 times a power of two per row and CTA that brings the largest into FP16's top
-//                 binade, fp32 as the sum of two FP16 columns (22 bits and more): what that drops lies 2^-39 and 2^-23 below the
-//                 row's largest value and the element, under what the fp32 sum keeps.  They are converted once into shared
-//                 memory and serve every weight row of the CTA.
+//                 binade, fp32 as the sum of two FP16 columns (22 bits and more).  An element is off by at most 2^-39 of its row's
+//                 largest, fp32 by 2^-23 of itself besides: under what the fp32 sum keeps as long as the largest elements have a
+//                 part in it.  In a sum that the weights leave to elements 2^25 times smaller (theirs being 0), it shows: the
+//                 price of one scale a row.  Converted once into shared memory, they serve every weight row of the CTA.
 //   split         a cluster of 1, 2, 4 or 8 CTAs takes a share of the weight rows, its CTAs a share of K each; in a CTA the warps
 //                 are groups with rows of their own, whose 1 to 8 warps share the CTA's K again.  Shared sums meet in shared
 //                 memory and distributed shared memory: no workspace, one launch, an order of additions that depends on the

@@ -7,7 +7,7 @@ import pytest
 
 torch = pytest.importorskip("torch")
 
-from test_decode4 import BAD_BATCH, Setup, c_batch, c_cache, calls, check_attention, e4m3_table, matvec_case, random_nvfp4, rotated64, stored64, values64, _p  # noqa: E402
+from test_decode4 import BAD_BATCH, Setup, T, c_batch, c_cache, calls, check_attention, e4m3_table, matvec_case, random_nvfp4, rotated64, stored64, values64, _p  # noqa: E402
 
 
 # ------------------------------------------------------------------------------------------------ refusals, without a GPU
@@ -66,6 +66,24 @@ def test_matvec_scales_from_any_byte_on(gpu, lb, N, K):
             got = torch.zeros(M, N, device="cuda")
             lb.nvfp4_matvec(x, w, inside, 0.5, got)
             assert torch.equal(got, want), (M, off)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("xt", ["bf16", "f32", "f16"])
+def test_matvec_elements_far_below_their_rows_largest(gpu, lb, xt):
+    """The largest elements meet weights of 0: what is left of the others is off by 2^-39 of the largest each (FP16: by nothing)."""
+    gen = torch.Generator("cuda").manual_seed(3)
+    w, ws = random_nvfp4((64, 512), gen)
+    w[:, ::16] = 0  # codes of k = 0, 1, 32, 33, ..
+    for far in (0, 10, 20, 30):
+        x = torch.randn(4, 512, device="cuda", generator=gen)
+        x.unflatten(1, (-1, 32))[:, :, :2] *= 2.0 ** (min(far, 14) if xt == "f16" else far)
+        x = x.to(T[xt])
+        y = torch.zeros(4, 64, device="cuda")
+        lb.nvfp4_matvec(x, w, ws, 1.0, y)
+        x64, w64 = x.double(), values64(w, ws)
+        tol = 2.0 ** -23 * (512 / 16 + 64) * (x64.abs() @ w64.abs().t()) + (xt != "f16") * 2.0 ** -39 * x64.abs().amax(1, keepdim=True) * w64.abs().sum(1)
+        assert ((y.double() - x64 @ w64.t()).abs() <= tol).all(), far
 
 
 # ------------------------------------------------------------------------------------------------ batches against the rules
