@@ -49,6 +49,20 @@ def test_matvec_longest_reductions(gpu, lb, M, K, xt):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("M,N,K,xt", [(16, 34979, 5120, "f16"), (32, 34979, 5120, "bf16"), (16, 34979, 5120, "f32"), (1, 30011, 8208, "bf16"), (8, 70001, 2064, "f32"),
+                                      (4, 34979, 12304, "f32"), (20, 5123, 17408, "bf16"), (3, 20011, 17408, "f16"), (32, 1003, 17408, "f16"), (29, 517, 17408, "f32"),
+                                      (9, 5003, 12304, "f32")])
+def test_matvec_many_meetings_and_launches(gpu, lb, M, N, K, xt):
+    """More tiles than sums have room for, so that CTAs (and a CTA's warps) meet several times, with a rest; rows that take several launches.
+    Calls repeat bit for bit."""
+    x, w, ws, y = matvec_case(lb, M, N, K, xt, "f32")
+    for _ in range(5):
+        again = torch.zeros_like(y)
+        lb.nvfp4_matvec(x, w, ws, 0.37, again)
+        assert torch.equal(again, y)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("N,K", [(1, 16), (5, 16), (40, 16), (33, 48), (17, 272), (75, 1088), (64, 5120), (37, 3344)])
 def test_matvec_scales_from_any_byte_on(gpu, lb, N, K):
     """Scales inside a larger array, from every kind of byte on: as the same scales on a boundary, whatever lies around them."""
