@@ -1556,7 +1556,6 @@ extern "C" int ling_b200_kv4_attention(int device, const ling_b200_kv4* cache, c
     set_error("kv4_attention: a 16-byte aligned workspace of " + std::to_string(need) + " bytes expected");
     return LING_B200_ERR_ARG;
   }
-  if (batch->max_rows == 0) return LING_B200_OK;
   DeviceGuard guard;
   int sms = 0;
   if (const int r = enter_device(guard, device, g_devices, g_mutex, attention_init, &sms)) return r;

@@ -144,6 +144,21 @@ def test_append_and_read_record_sequences_that_no_row_meets(gpu, lb, what):
 
 
 @pytest.mark.gpu
+def test_rows_beyond_a_bound_of_none_are_recorded(gpu, lb):
+    """max_rows = 0 and a sequence with rows: outside the bounds, by every call; without rows there is nothing to record."""
+    for seqs, want in (([(3, 20), (0, 5)], BAD_BATCH), ([(0, 20), (0, 5)], 0)):
+        s = Setup(lb, seqs, 64, 1, 16, padded=5 - sum(r for r, _ in seqs))
+        s.max_rows = 0
+        x, q = torch.randn(5, 1, 64, device="cuda", generator=s.gen), torch.zeros(5, 2, 64, dtype=torch.bfloat16, device="cuda")
+        out, o, err = torch.full_like(x, 9.0), torch.full_like(q, 9.0), torch.zeros(3, dtype=torch.int32, device="cuda")
+        s.cache().append(s.batch(), x, x, err=err[:1])
+        s.cache().read(s.batch(), out, None, err=err[1:2])
+        work = torch.zeros(s.cache().attention_workspace_bytes(s.batch(), 2), dtype=torch.uint8, device="cuda")
+        s.cache().attention(s.batch(), q, o, 0.1, work, err=err[2:])
+        assert err.tolist() == [want] * 3 and (out == 9.0).all() and (o == 9.0).all()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("G", [2, 8, 40])
 @pytest.mark.parametrize("row0", DESCENDING)
 def test_attention_skips_a_batch_whose_row0_descends(gpu, lb, row0, G):
