@@ -31,7 +31,8 @@ the ranks, ~10 % completions and admissions per step through the page pool), ser
 the scheduler loop: ling-engine_b200/ling_serve_headless), mixed (a 4096-row prefill chunk through the NVFP4 prefill path -- DeltaNet mixers and feed-forward blocks --
 beside an 8-sequence verify step; roofline against the NVFP4 tensor rate measured in the same run), toy.  --micro gemm |
 nvfp4 | nvfp4-swiglu | gdn-chunk | gdn-layer times one kernel (gdn-layer: one DeltaNet layer's prefill mixer) alone on resident operands (the small cases the profiler captures;
-gdn-chunk takes its row count from --shape's first number).
+gdn-chunk takes its row count from --shape's first number).  --micro decode4: the cases of perf/operators.py (the decode layer in 4 bits),
+as calls from Python and replayed as a graph.
 
 Inputs are synthetic (seeded): they stand in for the reference's private replay workload, whose shapes they take.
 Weights are 26.4 GB, far larger than the 126 MB L2, so consecutive steps cannot hit in L2 (no flush between steps).
@@ -867,6 +868,44 @@ def run_micro_gemm(args):
                       "larger_than_l2": nbytes > 126e6, "pdl": args.pdl}), flush=True)
 
 
+def run_micro_decode4(args):
+    """The cases of perf/operators.py through the library's calls, a JSON line each: enqueued back to back, and the same calls replayed as
+    one graph (the kernels alone).  As many sets of inputs in turn as L2 cannot hold; the median of three runs."""
+    import torch
+    sys.path.insert(0, ROOT)
+    ops = importlib.import_module("perf.operators")
+    ops.own = True
+
+    def us(f, n):
+        for i in range(3):
+            f(i)
+        a, b = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+        torch.cuda.synchronize()
+        a.record()
+        for i in range(n):
+            f(i)
+        b.record()
+        torch.cuda.synchronize()
+        return a.elapsed_time(b) * 1e3 / n
+
+    for case in ops.listed():
+        w = ops.work(case)
+        n = max(1, min(48, int(3e8 // w["bytes"]) + 1))
+        sets = [ops.prepare(case, i) for i in range(n)]
+        for s in sets:
+            ops.run(s)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            for s in sets:
+                ops.run(s)
+        runs = [(us(lambda i: ops.run(sets[i % n]), 100), us(lambda i: graph.replay(), 1 + 100 // n) / n) for _ in range(3)]
+        called, kernels = (sorted(r[j] for r in runs)[1] for j in range(2))
+        print(json.dumps({"micro": case["name"], "sets_of_inputs": n, "us_called": called, "us_kernels": kernels, "GB_per_s": w["bytes"] / kernels / 1e3,
+                          "TFLOP_per_s": w["flops"] / kernels / 1e6}), flush=True)
+        del sets, graph
+        torch.cuda.empty_cache()
+
+
 def ctx_stage_bytes(lbm, n_seqs):
     # the host-written descriptor block: count, per-sequence records, parent / token / forced-argmax rows
     return 16 + ((n_seqs * 24 + 15) // 16) * 16 + 3 * n_seqs * 32 * 4
@@ -962,11 +1001,13 @@ def main():
     ap.add_argument("--systems", type=int, default=0, help="served64: prompts begin with one of this many shared system messages")
     ap.add_argument("--prefix-kv-mb", type=int, default=0, help="served64 with --systems: the prefix KV store's budget for saved states (0: store off)")
     ap.add_argument("--pool-pages", type=int, default=0, help="served64: KV page pool size (0: sized for the resident sessions)")
-    ap.add_argument("--micro", default="", choices=["", "gemm", "nvfp4", "nvfp4-swiglu", "gdn-chunk", "gdn-layer", "sparse-head"], help="time one kernel alone on resident operands")
+    ap.add_argument("--micro", default="", choices=["", "gemm", "nvfp4", "nvfp4-swiglu", "gdn-chunk", "gdn-layer", "sparse-head", "decode4"], help="time one kernel alone on resident operands")
     ap.add_argument("--shape", default="24,34816,5120", help="--micro gemm: rows,N,K (default: the gate|up projection)")
     ap.add_argument("--iters", type=int, default=20)
     args = ap.parse_args()
     rank, local_rank, world = dist_env()
+    if args.micro == "decode4":
+        return run_micro_decode4(args)
     if args.micro:
         return run_micro_gemm(args)
     if args.impl == "reference":
