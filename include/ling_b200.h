@@ -682,7 +682,8 @@ int ling_b200_draft_head_run_sparse(ling_b200_draft_head* h, int session, const 
                                     float* scores, int* n_selected, int* selected);
 
 /* ------------------------------------------------------------------------------------------------ a decode layer in 4 bits
- * No counterpart in the reference, whose decode path reads FP8 weights and a BF16 cache.  NVFP4 operands (E2M1 values two a byte,
+ * The product stands beside the reference's streaming products with NVFP4 weights (stream_gemm.cu:181-349: FP16 rows, weights tiled
+ * beforehand); a 4-bit cache has no counterpart there (its cache is BF16).  NVFP4 operands (E2M1 values two a byte,
  * the first in the low nibble; one E4M3 scale per 16 values) for one token to a prompt's rows: a product with a few rows, a
  * paged KV cache, attention over it.  Unlike the _host entry points these take DEVICE pointers and only enqueue on `stream` (a
  * cudaStream_t; NULL = the default stream): they allocate nothing, wait for nothing and may be captured into a graph.  All

@@ -6,7 +6,8 @@
 // found by comparisons alone.  A key's rotation, and its largest value over 6, are carried in double and brought to fp32 by rounding to
 // odd (the last bit set when anything was cut off), which keeps every comparison with a value of fewer bits what it is for the exact
 // number: neither codes nor scales depend on how fp32 would have rounded the rotation.  Where nothing turns, the quotient of an
-// fp32 value and 6 needs no such care: beside a middle of two E4M3 values it lies at least two thirds of an fp32 step from it.  Queries need no such care and turn in fp32.
+// fp32 value and 6 needs no such care: beside a middle of two E4M3 values it lies at least two thirds of an fp32 step from it.  Queries
+// need no such care and turn in fp32.
 #include <algorithm>
 #include <cfloat>
 
@@ -147,9 +148,10 @@ struct Split {
 // the threads, then a thread takes a group of 16 dims of one K or V vector at a time (the groups of a vector are neighbouring lanes
 // of one warp), then 16 pairs of dims of a query that turn together, then 16 bytes of the queries' dims that do not turn.  What a
 // warp executes is of one kind: a query's turning dims beside its resting ones, lane by lane, cost three times the instructions.
-// Bound by the rows' bytes at many rows (they are read once, the queries written once, 9 / 16 byte a value goes to the cache), by
-// the chain row0 -> slot -> page -> store and a cosine in double at few.  Measured: 8192 rows of 32 + 2 x 8 heads
-// of 128 dims, all turning, BF16: 56 us, 3.2 TB/s; 64 rows of 24 + 2 x 4 heads of 256, 64 turning: 5 us.
+// Bound by L1 and shared memory at many rows (76 % busy: the angles in double and fp32 beside the rows; issue slots 54 %, DRAM 27 %; the
+// rows are read once, the queries written once, 9 / 16 byte a value goes to the cache), by the chain row0 -> slot -> page -> store
+// and a cosine in double at few.  Measured: 8192 rows of 32 + 2 x 8 heads of 128 dims, all turning, BF16: 57 us, 3.2 TB/s; 64 rows of
+// 24 + 2 x 4 heads of 256, 64 turning: 5 us.
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(kThreads) kv4_append_kernel(AppendArgs a, int chunk) {
   pdl_sync();  // first statement: see common.cuh
@@ -313,7 +315,8 @@ struct ReadArgs {
   int* err;
 };
 
-// As the append, the other way: a thread per group of 16 dims, read, decoded and stored.  8192 rows of 8 heads of 128 dims to BF16: 15 us.
+// As the append, the other way: a thread per group of 16 dims, read, decoded and stored.  8192 rows of 8 heads of 128 dims to BF16: 14 us,
+// 3 TB/s; the loads wait for the lookups and one another (issue slots 61 %, L1 48 % busy), 1024 blocks are 1.7 waves.
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(kThreads) kv4_read_kernel(ReadArgs a, int chunk) {
   pdl_sync();  // first statement: see common.cuh

@@ -50,9 +50,10 @@ struct AttnArgs {
 //                 worker: a CTA, whose warps take its steps in turn and add their results in shared memory, or (kSolo) a warp on
 //                 its own, which meets nobody.  An item that several workers share leaves partial results (O, m, l), which a
 //                 second kernel, launched dependent so that its start overlaps the first one's end, adds in order.
-// Measured, both kernels: one token over 128k positions (24 query heads on 4 kv heads of 256) 48 us, 3.1 TB/s of cache read; 64 tokens
-// over 1k to 8k positions (32 on 8 of 128) 101 us, 3.5 TB/s (6.5 TB/s is a plain copy).  What bounds it there is issue: codes to FP16
-// and their scales take as many slots as the MMAs.  8k positions 13 us: a launch, the plan, one ring's latency, the meeting, the join.
+// Measured, both kernels: one token over 128k positions (24 query heads on 4 kv heads of 256) 48.5 us, 3.1 TB/s of cache read; 64 tokens
+// over 1k to 8k positions (32 on 8 of 128) 102 us, 3.5 TB/s, over up to 64k (24 on 4 of 256) 648 us, 3.9 TB/s (6.5 TB/s is a plain copy).
+// No unit is full there (issue slots 40 to 48 % busy, DRAM 39 to 43 %, tensor pipe 18 to 21 %): two warps a scheduler wait for their own
+// conversions and MMAs.  8k positions 15 us: a launch, the plan, one ring's latency, the meeting, the join.
 constexpr int kDecRows = 8, kDecMaxCtas = 160;
 constexpr int kDecWarps = 8, kDecThreads = kDecWarps * 32, kDecMaxWorkers = kDecMaxCtas * kDecWarps;
 // Items from which warps work alone.  Measured, meeting / alone, 4 kv heads: 48 items of 8k positions 31 / 36 us, 64 items 41 / 41,
@@ -793,11 +794,12 @@ __global__ void __launch_bounds__(kJoinThreads) kv4_join_kernel(AttnArgs a) {
 //   warps 0..7   a thread half a row (its TMEM lane, 64 of the tile's keys): maximum, probabilities to FP16 in TMEM, in the place of
 //                the scores, as the value product's A operand; sum.  O is scaled in TMEM only when a score exceeds the row's
 //                reference by 2^kLazy, so that a tile's softmax need not wait for the tile before.
-// What bounds it is shared memory: operands are read once by the MMAs and written once by the converting warps (D = 256: 192 KB
-// and 128 KB a tile, 2560 cycles at 128 bytes, against 2048 cycles of MMA).  Measured (24 query heads on 4 kv heads of 256): 4096 rows
-// behind 4096 positions 757 us, 817 TFLOP/s (1644 is a library GEMM's rate); 4 trees of 20 rows behind up to 8k positions 48 us, of
-// which nearly 20 go into a CTA's first keys, its queries' conversion and its last rows.  A ring of pieces for K and V, with or
-// without warps of their own for each, was slower (840 and 909 us): more overlap only meets at shared memory.
+// Measured (24 query heads on 4 kv heads of 256): 4096 rows behind 4096 positions 758 us, 816 TFLOP/s (1644 is a library GEMM's rate), 5100
+// cycles a tile; the MMAs are 2048 of them (tensor pipe 40 % busy).  Operands are read once by the MMAs and written once by the
+// converting warps (D = 256: 192 KB and 128 KB a tile, 2560 cycles at 128 bytes; L1 and shared memory 79 % busy with that and the codes'
+// loads), and K and V have one buffer each, so that conversions and MMAs take turns.  4 trees of 20 rows behind up to 8k positions 48 us,
+// of which nearly 20 go into a CTA's first keys, its queries' conversion and its last rows.  A ring of pieces for K and V, with
+// or without warps of their own for each, was slower (840 and 909 us).
 // Every wait is bounded; one that runs out is recorded and the CTA leaves with its TMEM freed.
 constexpr int kTileRows = 128, kTileKeys = 128, kTileWarps = 17, kTileThreads = kTileWarps * 32, kTileWorkers = 256, kTileMarks = 8;
 constexpr int kMmaWarp = 16, kTileChain = kTileChainKeys / kTileKeys;  // tiles of a chain of value products

@@ -1,7 +1,8 @@
 // nvfp4_matvec.cu -- a few rows of activations times an NVFP4 weight matrix, activations in their own type:
 //   y[m][n] = alpha * sum_k x[m][k] * e2m1(values[n][k]) * e4m3(scales[n][k / 16])
-// for one token to a draft tree's 32 rows.  The weights are read once, N * K * 9 / 16 bytes: at these row counts that
-// stream is the floor (the prefill chunk's GEMM in nvfp4.cu pays a 128-row tile and an activation quantizer instead).
+// for one token to a draft tree's 32 rows.  A launch reads the weights once, N * K * 9 / 16 bytes: at these row counts that
+// stream is the floor (the prefill chunk's GEMM in nvfp4.cu pays a 128-row tile and an activation quantizer instead).  Rows whose
+// activations do not fit beside the others' (matvec_rows) are launches of their own.
 //
 //   tensor cores  mma.sync m16n8k16 in FP16 with fp32 sums: 16 weight rows are the MMA's M, 8 activation columns its N.  A thread
 //                 builds its A fragments in registers from the codes as the matrix holds them: 32 neighbouring codes of a
@@ -18,9 +19,10 @@
 //                 shape alone.  Many rows want no meeting (head: a warp per row pair), few rows many hands.
 //   loads         every warp streams 32 rows x 256 k (4.5 KB) at a time by cp.async through a private ring, across its rows;
 //                 nothing waits for another warp between meetings.
-// Measured, one BF16 row: 1024 x 5120 5.3 us; 5120 x 17408 22 us, 2.3 TB/s; 34816 x 5120 26 us, 3.8 TB/s; 248320 x 5120 153 us, 4.7 TB/s
-// (6.5 TB/s is a plain copy).  34816 x 5120: 8 rows 26 us, 16 rows 43 us, 32 rows 88 us.  Up to 8 rows the weights' stream and the
-// meetings bound it, beyond them a warp's instructions: two warps a scheduler do not hide the MMAs' and conversions' latencies.
+// Measured, one BF16 row: 1024 x 5120 5.5 us; 5120 x 17408 22 us, 2.3 TB/s; 34816 x 5120 27 us, 3.8 TB/s; 248320 x 5120 155 us, 4.6 TB/s
+// (6.5 TB/s is a plain copy).  34816 x 5120: 8 rows 32 us, 16 rows 44 us, 32 rows 94 us, 32 fp32 rows (two launches) 182 us.  No unit
+// is full (head: DRAM 53 %, issue slots 50 %, tensor pipe 24 % busy; 16 rows: 28, 36 and 29 %): two warps a scheduler do not hide the
+// latencies of MMAs and conversions, and where CTAs share K the meetings and unequal shares come on top.
 #include <algorithm>
 
 #include <cooperative_groups.h>
@@ -60,9 +62,6 @@ __device__ __forceinline__ void cp16(uint32_t dst, const void* src, int bytes) {
 }
 __device__ __forceinline__ void cp8(uint32_t dst, const void* src, int bytes) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void cp4(uint32_t dst, const void* src, int bytes) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -529,8 +528,8 @@ int matvec_launch(MatvecArgs a, const Split& split, cudaStream_t s) {
   LB_LAUNCH("nvfp4_matvec_kernel");
   return LING_B200_OK;
 }
-// As many rows a launch as their activations fit beside the weights' rings: at K = 5120 32 columns, at 17408 25 (in 4 tiles; the rows left
-// over are launches of their own, which read the weights again).
+// As many rows a launch as their activations fit beside the weights' rings, in 1, 2 or 4 tiles of 8 columns: at K = 5120 32 columns, at
+// 17408 up to 25 at once, more as 16 and 16.
 template <typename TX>
 int matvec_rows(MatvecArgs a, int device, cudaStream_t s) {
   constexpr int kCols = sizeof(TX) == 4 ? 2 : 1;
