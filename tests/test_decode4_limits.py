@@ -275,3 +275,22 @@ def test_attention_scores_that_grow_from_chain_to_chain(gpu, lb, seqs, G):
     _, out, _ = check_attention(lb, s, "bf16", G, spread=2.0, lse=False)
     last = seqs[-1][0]
     assert torch.isnan(out[-last:]).all() and torch.isfinite(out[:-last]).all()
+
+
+# ------------------------------------------------------------------------------------------------ lopsided batches
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 256])
+def test_attention_one_long_context_among_empty_sequences(gpu, lb, D):
+    """Bounds that speak for many items, and one item: its context is shared by hundreds of warps."""
+    s = Setup(lb, [(0, 3)] * 50 + [(1, 120000)] + [(0, 0)] * 49, D, 1, 64, seed=31, padded=1)
+    check_attention(lb, s, "bf16", 3, spread=2.0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("G", [1, 8])
+@pytest.mark.parametrize("bad", [0, 20, 39, 69])
+def test_attention_records_a_bad_sequence_among_many(gpu, lb, bad, G):
+    """Wherever it stands, by either kernel; the others get their results."""
+    s = Setup(lb, [(1 + i % 7, 40 + 13 * i) for i in range(70)], 64, 1, 16, seed=32)
+    s.slot[bad] = s.tables.shape[0]
+    check_attention(lb, s, "bf16", G, err_code=BAD_BATCH, skip=[bad])
